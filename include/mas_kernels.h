@@ -9,6 +9,9 @@
  * embedding gather, and paged attention over the KV cache: split-KV decode and causal context
  * (prefill), each optionally writing the o_proj input's fp8 quantize.
  *
+ * Also: a KV cache held in 4 bits (microscaling fp4) - the append that quantizes, its inverse, decode and
+ * context attention over it - and a step's index tensors built from its rows' lengths.
+ *
  * Conventions shared by every entry point:
  *   - Pointers are device pointers; tensors are bf16 unless stated (bf16 travels as raw 16-bit
  *     words, fp8 as raw bytes). Strides are in ELEMENTS of the pointed-to type, and the last
@@ -50,11 +53,13 @@ extern "C" {
 #define MAS_ERRBIT_TOKEN_ID 1u  /* embedding: id < 0 or id >= vocab                       */
 #define MAS_ERRBIT_POSITION 2u  /* rope: position < 0 or >= table rows; kv: position < 0;
                                    attention: seq_len out of range, or (context) a row with
-                                   more query tokens than max_q_len                         */
+                                   more query tokens than max_q_len; plan: a row's lengths
+                                   negative or past its block table                         */
 #define MAS_ERRBIT_BATCH 4u     /* kv: batch index outside [0, batch)                     */
 #define MAS_ERRBIT_PAGE 8u      /* kv: page slot past kv_indices or page id out of range  */
 #define MAS_ERRBIT_SLOT 16u     /* kv slot form: slot >= num_pages * page_size            */
 #define MAS_ERRBIT_PLACEHOLDER 32u /* embedding: placeholder -1 - r with r >= num_last     */
+#define MAS_ERRBIT_POOL 64u     /* plan: free pages or token count do not reach all rows  */
 
 /* Library version, (major << 16) | (minor << 8) | patch: of this header, and of the library loaded. A
    change to a function's signature or to a constant's meaning changes it. */
@@ -348,6 +353,114 @@ int64_t mas_paged_decode_attention_workspace_bytes(int64_t batch, int64_t num_q_
  */
 int64_t mas_paged_context_attention_workspace_bytes(int64_t num_rows, int64_t max_q_len, int64_t num_q_heads,
                                                     int64_t num_kv_heads, int64_t head_dim);
+
+/*
+ * ---- The 4-bit KV cache ----
+ * A head's row of head_dim elements (a multiple of 32) is cut into blocks of 32. A block is stored as 32
+ * e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives: sign, 2 exponent bits, 1 mantissa bit), two a
+ * byte with the even element in the low half, and one power of two, a byte s standing for 2^(s - 127) (255:
+ * NaN). The code of element i of block j of head h at (page, entry) is in byte
+ *   cache + page*page_stride + entry*entry_stride + h*head_stride + 16*j + i/2,
+ * the block's power in byte
+ *   scale + page*scale_page_stride + h*scale_head_stride + j*page_size + entry.
+ * Strides are in BYTES. page_size: a power of two of at least 16. Codes and their strides: 16-byte
+ * aligned, powers and theirs 4-byte aligned. 4.25 bits an element.
+ * No counterpart in the reference (its cache is bf16, model_runner.py:83-85).
+ */
+
+/*
+ * Paged KV-cache append into the 4-bit cache, block-table form: destinations as for
+ * mas_append_paged_kv_cache_bf16. For each block, s is the smallest byte under which max |x| < 7 * 2^(s - 127)
+ * (255 where the block holds a NaN or an infinity, its codes then 0), and each code the nearest one to
+ * x / 2^(s - 127), ties to the even code: off by at most half a step. The bits follow from the inputs alone.
+ * Duplicate destinations are allowed (what they hold then may mix the writers' blocks).
+ */
+int mas_append_paged_kv_cache_fp4(void* k_cache, void* v_cache, int64_t page_stride, int64_t entry_stride,
+                                  int64_t head_stride, void* k_scale, void* v_scale, int64_t scale_page_stride,
+                                  int64_t scale_head_stride, int64_t num_pages, int64_t page_size, const void* key,
+                                  int64_t key_stride, int64_t key_head_stride, const void* value,
+                                  int64_t value_stride, int64_t value_head_stride, const int32_t* batch_indices,
+                                  const int32_t* positions, const int32_t* kv_indices, int64_t num_indices,
+                                  const int32_t* kv_indptr, int64_t batch, int64_t rows, int64_t num_heads,
+                                  int64_t head_dim, uint32_t* err, hipStream_t stream);
+
+/* The same, slot-mapping form (destinations as for mas_store_kv_slots_bf16). */
+int mas_store_kv_slots_fp4(void* k_cache, void* v_cache, int64_t page_stride, int64_t entry_stride,
+                           int64_t head_stride, void* k_scale, void* v_scale, int64_t scale_page_stride,
+                           int64_t scale_head_stride, int64_t num_pages, int64_t page_size, const void* key,
+                           int64_t key_stride, int64_t key_head_stride, const void* value, int64_t value_stride,
+                           int64_t value_head_stride, const int64_t* slot_mapping, int64_t rows, int64_t num_heads,
+                           int64_t head_dim, uint32_t* err, hipStream_t stream);
+
+/*
+ * Rows of the 4-bit cache as bf16, the inverse of the slot form: key[t, h, :] and value[t, h, :] become the
+ * values that slot slot_mapping[t]'s codes stand for, exactly. A negative slot gives zeros, so does one past
+ * the cache (MAS_ERRBIT_SLOT).
+ */
+int mas_load_kv_slots_fp4(void* key, int64_t key_stride, int64_t key_head_stride, void* value, int64_t value_stride,
+                          int64_t value_head_stride, const void* k_cache, const void* v_cache, int64_t page_stride,
+                          int64_t entry_stride, int64_t head_stride, const void* k_scale, const void* v_scale,
+                          int64_t scale_page_stride, int64_t scale_head_stride, int64_t num_pages, int64_t page_size,
+                          const int64_t* slot_mapping, int64_t rows, int64_t num_heads, int64_t head_dim,
+                          uint32_t* err, hipStream_t stream);
+
+/*
+ * Paged decode attention over the 4-bit cache: mas_paged_decode_attention_bf16 with the keys and values that
+ * the codes stand for (its shapes, masks, errors, workspace and outputs; page_size at least 16). Workspace
+ * bytes: mas_paged_decode_attention_workspace_bytes.
+ */
+int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int64_t out_head_stride, const void* q,
+                                   int64_t q_stride, int64_t q_head_stride, const void* k_cache, const void* v_cache,
+                                   int64_t page_stride, int64_t entry_stride, int64_t head_stride,
+                                   const void* k_scale, const void* v_scale, int64_t scale_page_stride,
+                                   int64_t scale_head_stride, int64_t num_pages, int64_t page_size,
+                                   const int32_t* block_tables, int64_t block_table_stride, int64_t max_blocks,
+                                   const int32_t* seq_lens, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                   int64_t head_dim, float bmm1_scale, float bmm2_scale, int out_fp8,
+                                   const float* out_scale_dev, float out_scale_host, void* workspace,
+                                   int64_t workspace_bytes, uint32_t* err, hipStream_t stream);
+
+/*
+ * Paged causal attention of prompt rows over the 4-bit cache: mas_paged_context_attention_bf16 with the keys
+ * and values that the codes stand for (its shapes, masks, workspace and outputs; page_size at least 16). Positions
+ * on a page id outside the cache enter as zero keys and values (MAS_ERRBIT_PAGE).
+ */
+int mas_paged_context_attention_fp4(void* out, int64_t out_stride, int64_t out_head_stride, const void* q,
+                                    int64_t q_stride, int64_t q_head_stride, const void* k_cache, const void* v_cache,
+                                    int64_t page_stride, int64_t entry_stride, int64_t head_stride,
+                                    const void* k_scale, const void* v_scale, int64_t scale_page_stride,
+                                    int64_t scale_head_stride, int64_t num_pages, int64_t page_size,
+                                    const int32_t* block_tables, int64_t block_table_stride, int64_t max_blocks,
+                                    const int32_t* seq_lens, const int32_t* cu_seqlens_q, int64_t num_rows,
+                                    int64_t max_q_len, int64_t max_kv_len, int64_t num_q_heads, int64_t num_kv_heads,
+                                    int64_t head_dim, float bmm1_scale, float bmm2_scale, int out_fp8,
+                                    const float* out_scale_dev, float out_scale_host, void* workspace,
+                                    int64_t workspace_bytes, uint32_t* err, hipStream_t stream);
+
+/*
+ * A step's index tensors from its rows' lengths. Row r (rows in order) holds cached_lens[r] positions and gets
+ * new_lens[r] tokens:
+ *   cu_seqlens_q [rows + 1]: 0 and the running sums of the rows' tokens; seq_lens[r] = cached + new;
+ *   token t < num_tokens of row r (cu_seqlens_q[r] <= t < cu_seqlens_q[r + 1]): positions[t] = p =
+ *   cached_lens[r] + t - cu_seqlens_q[r], batch_indices[t] = r, slot_mapping[t] = page * page_size +
+ *   p % page_size with page = block_tables[r, p / page_size];
+ *   tokens past the last row's: position 0, batch index -1, slot -1 (padding, skipped by the slot form of the stores).
+ * The pages of blocks ceil(cached / page_size) .. ceil((cached + new) / page_size) - 1 of row r are taken in row
+ * order from the ring free_pages [num_free_pages] - free_range = {head, tail} (int64, counting up; entry i of the
+ * ring is free_pages[i % num_free_pages], entries head .. tail - 1 are free) - and written to its block table;
+ * free_range_out = {head + pages taken, tail}.
+ * From the first row on whose tokens pass num_tokens or whose pages pass the free ones, rows get no token
+ * (MAS_ERRBIT_POOL; their lengths and tables stay). A row with a negative length, or one past
+ * max_blocks * page_size, is passed over alone (MAS_ERRBIT_POSITION). A negative page in a table gives slot -1
+ * (MAS_ERRBIT_PAGE). seq_lens and free_range_out must not be the lengths' and the range's own memory.
+ * Replaces the fill loops of ModelRunner.prepare (miniagentserve/engine/model_runner.py:194-221) and the page
+ * hand-out of KVBlockManager.allocate (miniagentserve/engine/block_manager.py:43-73) for steps planned on the GPU.
+ */
+int mas_plan_step(int32_t* positions, int32_t* batch_indices, int64_t* slot_mapping, int32_t* cu_seqlens_q,
+                  int32_t* seq_lens, int64_t* free_range_out, int32_t* block_tables, int64_t block_table_stride,
+                  int64_t max_blocks, const int32_t* new_lens, const int32_t* cached_lens, int64_t rows,
+                  const int32_t* free_pages, int64_t num_free_pages, const int64_t* free_range, int64_t page_size,
+                  int64_t num_tokens, uint32_t* err, hipStream_t stream);
 
 #ifdef __cplusplus
 }

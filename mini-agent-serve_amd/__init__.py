@@ -16,6 +16,13 @@ Drop-ins for the calls the reference's layer modules make
 - ``fused.apply_rope_and_append_paged_kv_cache``                    (:163-166 + :170-173 + the llama-4
   query scale at :175-179, one kernel)
 
+Around a KV cache held in 4 bits (no counterpart in the reference, whose cache is bf16):
+
+- ``page.fp4_kv_cache``, ``page.append_paged_kv_cache_fp4``, ``page.store_kv_slots_fp4``, ``page.load_kv_slots_fp4``
+- ``attention.batch_decode_with_fp4_kv_cache``, ``attention.batch_context_with_fp4_kv_cache``
+- ``step.plan_step``: a step's index tensors and pages from its rows' lengths
+  (ModelRunner.prepare, miniagentserve/engine/model_runner.py:176-225), for any cache
+
 Each op validates its tensors, then calls hand-written HIP kernels in ``libmas_kernels.so``
 through the C ABI of ``include/mas_kernels.h`` on torch's current stream. There is no CPU or
 PyTorch fallback: without the built library every op raises.
@@ -25,7 +32,7 @@ imports it as ``mini_agent_serve_amd``.
 """
 from __future__ import annotations
 
-from . import _compile_fix, _lib, activation, attention, embedding, fused, norm, page, rope, workloads
+from . import _compile_fix, _lib, activation, attention, embedding, fused, norm, page, rope, step, workloads
 from . import layer_pass
 from . import _ops  # noqa: F401  (registers the torch.library ops)
 
@@ -34,13 +41,16 @@ from .activation import silu_and_mul, silu_and_mul_quant
 from .embedding import Embedding
 from .fused import apply_rope_and_append_paged_kv_cache
 from .norm import fused_add_rmsnorm, fused_add_rmsnorm_quant
-from .page import append_paged_kv_cache, store_kv_slots
+from .page import (append_paged_kv_cache, append_paged_kv_cache_fp4, fp4_kv_cache, load_kv_slots_fp4, store_kv_slots,
+                   store_kv_slots_fp4)
 from .rope import apply_rope_with_cos_sin_cache_inplace
+from .step import plan_step
 
 __all__ = [
-    "activation", "attention", "embedding", "fused", "norm", "page", "rope", "workloads", "layer_pass",
+    "activation", "attention", "embedding", "fused", "norm", "page", "rope", "step", "workloads", "layer_pass",
     "apply_rope_and_append_paged_kv_cache",
     "silu_and_mul", "silu_and_mul_quant", "Embedding", "fused_add_rmsnorm", "fused_add_rmsnorm_quant", "append_paged_kv_cache",
+    "append_paged_kv_cache_fp4", "store_kv_slots_fp4", "load_kv_slots_fp4", "fp4_kv_cache", "plan_step",
     "store_kv_slots", "apply_rope_with_cos_sin_cache_inplace", "load_library", "library_version",
 ]
 

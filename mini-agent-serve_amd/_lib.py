@@ -7,6 +7,7 @@ machine without the built library every op raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.util
 import sys
@@ -61,6 +62,28 @@ _SIGNATURES: dict[str, list] = {
                                          _i64, _i64, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64,
                                          _i64, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_float, _i32, _c_void_p,
                                          ctypes.c_float, _c_void_p, _i64, _c_void_p, _c_void_p],
+    "mas_append_paged_kv_cache_fp4": [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64,
+                                      _i64, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,
+                                      _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64,
+                                      _i64, _c_void_p, _c_void_p],
+    "mas_store_kv_slots_fp4": [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64,
+                               _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64,
+                               _i64, _i64, _c_void_p, _c_void_p],
+    "mas_load_kv_slots_fp4": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64,
+                              _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _i64,
+                              _i64, _c_void_p, _c_void_p],
+    "mas_paged_decode_attention_fp4": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                       _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64,
+                                       _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _i64, _f32, _f32,
+                                       _i32, _c_void_p, _f32, _c_void_p, _i64, _c_void_p, _c_void_p],
+    "mas_paged_context_attention_fp4": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                        _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64,
+                                        _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64,
+                                        _i64, _i64, _f32, _f32, _i32, _c_void_p, _f32, _c_void_p, _i64,
+                                        _c_void_p, _c_void_p],
+    "mas_plan_step": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
+                      _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p,
+                      _c_void_p],
 }
 _RESTYPES = {"mas_status_string": ctypes.c_char_p, "mas_paged_decode_attention_workspace_bytes": ctypes.c_int64,
              "mas_paged_context_attention_workspace_bytes": ctypes.c_int64}
@@ -72,6 +95,7 @@ ERROR_BITS = {
     8: "page slot past kv_indices or page id outside the cache",
     16: "slot past the end of the cache",
     32: "placeholder -1 - r past the previous step's samples",
+    64: "free pages or token count too few for all rows",
 }
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -150,3 +174,12 @@ def stream_handle(device: torch.device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_STAY = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one: the launches and device queries of a call go to the
+    tensors' GPU, whichever is current."""
+    return _STAY if device.index == torch.cuda.current_device() else torch.cuda.device(device)

@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 from torch.library import custom_op
 
-from . import activation, attention, embedding, fused, norm, page, rope
+from . import activation, attention, embedding, fused, norm, page, rope, step
 
 Tensor = torch.Tensor
 
@@ -250,4 +250,87 @@ def _silu_and_mul_quant_hs(input: Tensor, out: Tensor, scale: float) -> None:
 
 @_silu_and_mul_quant_hs.register_fake
 def _(input, out, scale):
+    return None
+
+
+@custom_op("mas::append_paged_kv_cache_fp4", mutates_args=("k", "v", "k_scale", "v_scale", "error_flags"))
+def _append_paged_kv_cache_fp4(append_key: Tensor, append_value: Tensor, batch_indices: Tensor, positions: Tensor,
+                               k: Tensor, v: Tensor, k_scale: Tensor, v_scale: Tensor, kv_indices: Tensor,
+                               kv_indptr: Tensor, kv_layout: str, error_flags: Optional[Tensor]) -> None:
+    page._append_fp4(append_key, append_value, batch_indices, positions, (k, v, k_scale, v_scale), kv_indices,
+                     kv_indptr, kv_layout, error_flags)
+
+
+@_append_paged_kv_cache_fp4.register_fake
+def _(append_key, append_value, batch_indices, positions, k, v, k_scale, v_scale, kv_indices, kv_indptr, kv_layout,
+      error_flags):
+    return None
+
+
+@custom_op("mas::store_kv_slots_fp4", mutates_args=("k", "v", "k_scale", "v_scale", "error_flags"))
+def _store_kv_slots_fp4(key: Tensor, value: Tensor, k: Tensor, v: Tensor, k_scale: Tensor, v_scale: Tensor,
+                        slot_mapping: Tensor, kv_layout: str, error_flags: Optional[Tensor]) -> None:
+    page._slots_fp4("store", key, value, (k, v, k_scale, v_scale), slot_mapping, kv_layout, error_flags)
+
+
+@_store_kv_slots_fp4.register_fake
+def _(key, value, k, v, k_scale, v_scale, slot_mapping, kv_layout, error_flags):
+    return None
+
+
+@custom_op("mas::load_kv_slots_fp4", mutates_args=("key", "value", "error_flags"))
+def _load_kv_slots_fp4(key: Tensor, value: Tensor, k: Tensor, v: Tensor, k_scale: Tensor, v_scale: Tensor,
+                       slot_mapping: Tensor, kv_layout: str, error_flags: Optional[Tensor]) -> None:
+    page._slots_fp4("load", key, value, (k, v, k_scale, v_scale), slot_mapping, kv_layout, error_flags)
+
+
+@_load_kv_slots_fp4.register_fake
+def _(key, value, k, v, k_scale, v_scale, slot_mapping, kv_layout, error_flags):
+    return None
+
+
+@custom_op("mas::paged_decode_attention_fp4", mutates_args=("workspace", "out", "error_flags"))
+def _paged_decode_attention_fp4(query: Tensor, k: Tensor, v: Tensor, k_scale: Tensor, v_scale: Tensor,
+                                workspace: Tensor, block_tables: Tensor, seq_lens: Tensor, bmm1_scale: float,
+                                bmm2_scale: float, out: Tensor, kv_layout: str, quant_scale: Optional[Tensor],
+                                quant_scale_host: float, error_flags: Optional[Tensor]) -> None:
+    attention._decode_fp4(query, (k, v, k_scale, v_scale), workspace, block_tables, seq_lens, bmm1_scale, bmm2_scale,
+                          out, kv_layout, error_flags, _quant_scale(quant_scale, quant_scale_host))
+
+
+@_paged_decode_attention_fp4.register_fake
+def _(query, k, v, k_scale, v_scale, workspace, block_tables, seq_lens, bmm1_scale, bmm2_scale, out, kv_layout,
+      quant_scale, quant_scale_host, error_flags):
+    return None
+
+
+@custom_op("mas::paged_context_attention_fp4", mutates_args=("workspace", "out", "error_flags"))
+def _paged_context_attention_fp4(query: Tensor, k: Tensor, v: Tensor, k_scale: Tensor, v_scale: Tensor,
+                                 workspace: Optional[Tensor], block_tables: Tensor, seq_lens: Tensor,
+                                 cu_seqlens_q: Tensor, max_q_len: int, max_kv_len: int, bmm1_scale: float,
+                                 bmm2_scale: float, out: Tensor, kv_layout: str, quant_scale: Optional[Tensor],
+                                 quant_scale_host: float, error_flags: Optional[Tensor]) -> None:
+    attention._context_fp4(query, (k, v, k_scale, v_scale), workspace, block_tables, seq_lens, cu_seqlens_q, max_q_len,
+                           max_kv_len, bmm1_scale, bmm2_scale, out, kv_layout, error_flags,
+                           _quant_scale(quant_scale, quant_scale_host))
+
+
+@_paged_context_attention_fp4.register_fake
+def _(query, k, v, k_scale, v_scale, workspace, block_tables, seq_lens, cu_seqlens_q, max_q_len, max_kv_len,
+      bmm1_scale, bmm2_scale, out, kv_layout, quant_scale, quant_scale_host, error_flags):
+    return None
+
+
+@custom_op("mas::plan_step", mutates_args=("block_tables", "positions", "batch_indices", "slot_mapping",
+                                           "cu_seqlens_q", "seq_lens", "free_range_out", "error_flags"))
+def _plan_step(new_lens: Tensor, cached_lens: Tensor, block_tables: Tensor, free_pages: Tensor, free_range: Tensor,
+               page_size: int, positions: Tensor, batch_indices: Tensor, slot_mapping: Tensor, cu_seqlens_q: Tensor,
+               seq_lens: Tensor, free_range_out: Tensor, error_flags: Optional[Tensor]) -> None:
+    step._plan(new_lens, cached_lens, block_tables, free_pages, free_range, page_size,
+               (positions, batch_indices, slot_mapping, cu_seqlens_q, seq_lens, free_range_out), error_flags)
+
+
+@_plan_step.register_fake
+def _(new_lens, cached_lens, block_tables, free_pages, free_range, page_size, positions, batch_indices, slot_mapping,
+      cu_seqlens_q, seq_lens, free_range_out, error_flags):
     return None

@@ -41,8 +41,9 @@
 // sides on one card in one session; cards and sessions differ by up to 8%, so figures of different pairs
 // do not follow each other.)
 #include <algorithm>
+#include <type_traits>
 
-#include "device.h"
+#include "fp4.h"
 
 namespace mas {
 namespace {
@@ -127,6 +128,11 @@ struct ContextArgs {
   uint32_t* err;
 };
 
+// The same over the 4-bit cache of fp4_cache.hip (k_cache, v_cache and their strides are then unused).
+struct Fp4ContextArgs : ContextArgs {
+  Fp4Cache c;
+};
+
 // Wavefronts per workgroup (kWaves, 4 or 8): each stages its share of every key / value tile, and
 // all of them read it. The register allocation is capped for two wavefronts per SIMD (8 / kWaves
 // workgroups per CU, at most 256 VGPRs per lane). Eight wavefronts (two 32-token tiles of the same
@@ -170,6 +176,11 @@ constexpr int kWaitVmcnt0 = 0x0f70;
 constexpr int kPagesLane = 0, kPagesTile = 2;
 // kPagesMulti8 + i: pages of 8 << i slots (i < 3)
 constexpr int kPagesMulti8 = 4, kPagesMulti16 = 5, kPagesMulti32 = 6;
+//   kPagesFp4   - the 4-bit cache (pages of at least 16 slots): a lane loads 32 codes of a row and their power,
+//                 and decodes them to bf16 on the way into LDS, a tile after it loaded them.
+constexpr int kPagesFp4 = 8;
+template <int kPages>
+using ContextArgsOf = std::conditional_t<kPages == kPagesFp4, Fp4ContextArgs, ContextArgs>;
 
 // Key tiles per split of a token tile that reaches `ntiles` key tiles: its kv_splits splits share
 // them evenly, at least 4 each (fewer splits then hold them all). From the tile's own reach, not
@@ -518,7 +529,7 @@ __device__ __forceinline__ bool self_plan_item(const ContextArgs& a, int lane, i
 // kWork: how workgroups map to work (each a separate instance, so that the one-kernel instances
 // keep their code).
 template <int D, int kPages, int kWaves, int kWork>
-__global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextArgsOf<kPages> a) {
   constexpr bool kSplit = kWork == kWorkSplit;
   constexpr bool kPlan = kWork == kWorkPlan || kWork == kWorkSelfPlan;  // items from a plan
   constexpr int kCtxWaves = kWaves;
@@ -702,7 +713,7 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
   // this kv head, its records ending after the last position below kv_len (none for a page id outside
   // the cache): the rows past them arrive as zeros. A wavefront's rows lie in PPW pages. The host
   // keeps this mode to layouts whose in-page byte offsets fit 31 bits.
-  constexpr bool kMulti = kPages >= kPagesMulti8;
+  constexpr bool kMulti = kPages >= kPagesMulti8 && kPages <= kPagesMulti32;
   constexpr bool kDirect = kPages == kPagesTile || kMulti;
   constexpr int PS = kMulti ? (8 << (kPages - kPagesMulti8)) : kTileP;  // rows per page (kMulti)
   constexpr int RPI = 64 / CPR, NI = kTileP / RPI / kCtxWaves;
@@ -787,6 +798,99 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
   auto dma_values = [&](const TilePages& t, uint16_t* dst) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) dma_value(t, dst, j);
+  };
+
+  // ---- kPagesFp4: a tile's rows in chunks of 32 codes (16 bytes, one power byte), one chunk of a tensor per
+  // lane: with 256 chunks of keys and as many of values (head_dim 128) and 256 threads, each takes one of both;
+  // else a wavefront stages keys or values only (or, past the chunks, nothing). A wavefront's chunks lie in
+  // 16-row groups, each in one page.
+  constexpr bool kFp4 = kPages == kPagesFp4;
+  constexpr int FC = D / kFp4Block;               // chunks per row
+  constexpr int FK = kTileP * FC;                 // chunks per tile and tensor
+  constexpr bool kBoth = 2 * FK > kCtxThreads;    // a lane stages a chunk of each
+  constexpr int FG = FC == 4 ? 1 : 2;             // 16-row groups per wavefront
+  static_assert(!kFp4 || 2 * FK <= 2 * kCtxThreads, "a chunk of each tensor per lane, at most");
+  const int f_role = kBoth ? 0 : wave / (FK / 64);  // 0: keys (and values when kBoth), 1: values, 2: nothing
+  const int f_idx = tid % FK, f_row = f_idx / FC, f_chunk = f_idx % FC;
+  const int f_row0 = (wave % (FK / 64)) * (64 / FC);  // this wavefront's first row
+  struct Fp4Pages {  // the wavefront's 16-row groups: byte offsets of their first rows, and their valid rows
+    int64_t code[FG], power[FG];
+    int rows[FG];
+  };
+  struct Fp4Regs {
+    u32x4 w;
+    uint32_t power;
+    bool ok;
+  };
+  auto fp4_find = [&](int base, bool prologue, int limit) {
+    Fp4Pages t{};
+    if constexpr (kFp4) {
+      if (!prologue) {
+        const int chunk = chunk_of(base), next = chunk_of(base + kTileP);
+        if (chunk != page_chunk) {  // uniform
+          page_ids = next_page_ids;
+          page_chunk = chunk;
+        }
+        if (next != chunk) next_page_ids = load_page_ids(next);
+      }
+#pragma unroll
+      for (int g = 0; g < FG; ++g) {
+        const int pos = base + f_row0 + 16 * g, entry = pos >> a.log2_page;
+        const int rows = __builtin_amdgcn_readfirstlane(max(0, min(limit - pos, 16)));
+        const uint32_t page = static_cast<uint32_t>(prologue ? bt_const[min(entry, last_page)]
+                                                             : __builtin_amdgcn_readlane(page_ids, entry & 63));
+        const bool ok = page < pages_u32;
+        page_bad |= rows > 0 && !ok;
+        const int64_t pg = ok ? page : 0u;
+        t.code[g] = pg * a.c.page_stride + static_cast<int64_t>(pos & pmask) * a.c.entry_stride;
+        t.power[g] = pg * a.c.scale_page_stride + (pos & pmask);
+        t.rows[g] = ok ? rows : 0;
+      }
+    }
+    return t;
+  };
+  auto fp4_issue = [&](const Fp4Pages& t, bool values) {
+    Fp4Regs x{};
+    if constexpr (kFp4) {
+      const int g = FG == 1 ? 0 : lane >> 5, row = f_row & 15;
+      const int64_t code = FG == 1 || g == 0 ? t.code[0] : t.code[FG - 1];
+      const int64_t power = FG == 1 || g == 0 ? t.power[0] : t.power[FG - 1];
+      const int rows = FG == 1 || g == 0 ? t.rows[0] : t.rows[FG - 1];
+      const uint8_t* src = (values ? a.c.v : a.c.k) + kvh * a.c.head_stride + code;
+      const uint8_t* psrc = (values ? a.c.v_scale : a.c.k_scale) + kvh * a.c.scale_head_stride + power;
+      x.w = load_cached(src + (static_cast<uint32_t>(row) * static_cast<uint32_t>(a.c.entry_stride) + 16u * f_chunk));
+      x.power = psrc[static_cast<uint32_t>(f_chunk) * static_cast<uint32_t>(a.c.page_size) + row];
+      x.ok = row < rows;
+    }
+    return x;
+  };
+  // Piece i (of four, 8 elements each) of a chunk into its place in a tile buffer. Values take the pieces in an
+  // order turned by the row (fp4_turn), so that the 16 lanes of a store's phase, four rows of four chunks, hit all
+  // 16 slots of the banks; a key row's swizzle alone does that.
+  auto fp4_turn = [&](Fp4Regs& x, bool values) {
+    if constexpr (kFp4) {
+      if (!x.ok) {  // past the sequence, or on a bad page: zeros
+        x.w = u32x4{0u, 0u, 0u, 0u};
+        x.power = 0u;
+      }
+      if (values) {
+        const bool t1 = f_row & 1, t2 = f_row & 2;
+        x.w = t1 ? u32x4{x.w[1], x.w[0], x.w[3], x.w[2]} : x.w;
+        x.w = t2 ? u32x4{x.w[2], x.w[3], x.w[0], x.w[1]} : x.w;
+      }
+    }
+  };
+  const int f_key_at = f_row * D + 8 * ((4 * f_chunk) ^ key_swizzle(f_row));
+  const int f_value_at = f_row * D + 8 * ((4 * f_chunk) ^ value_swizzle(f_row) ^ (f_row & 3));
+  auto fp4_put = [&](const Fp4Regs& x, uint16_t* dst, bool values, int i) {
+    if constexpr (kFp4)
+      *reinterpret_cast<u32x4*>(dst + ((values ? f_value_at : f_key_at) ^ 8 * i)) =
+          fp4x8_decode(x.w[i], __uint_as_float(x.power << 23));
+  };
+  auto fp4_stage = [&](Fp4Regs& x, uint16_t* dst, bool values) {
+    fp4_turn(x, values);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fp4_put(x, dst, values, i);
   };
 
   // kPagesLane: each lane reads the page of each of its rows; rows past kv_len load the sequence's
@@ -947,7 +1051,38 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
   f32x16 s_even{}, s_odd{};   // the scores of a tile's halves
   bf16x8 pb_even[2], pb_odd[2];  // and their weights
   TilePages ahead{};  // kDirect: the pages of the tile whose keys the DMA took last
+  // kPagesFp4: in step it the lane holds the codes of tile it + 2's keys and of tile it + 1's values, loaded a
+  // step before (f_k and f_v; the only ones in f_k where the lane stages one tensor), and f_ahead the pages of
+  // the tile whose keys were loaded last.
+  Fp4Regs f_k{}, f_v{};
+  Fp4Pages f_ahead{};
+  const auto f_limit = [&](int tile) { return tile < it_end ? kv_len : 0; };
   if (it_begin < it_end) {
+    if constexpr (kFp4) {
+      const Fp4Pages p0 = fp4_find(it_begin * kTileP, true, kv_len);
+      const Fp4Pages p1 = fp4_find((it_begin + 1) * kTileP, true, f_limit(it_begin + 1));
+      f_ahead = fp4_find((it_begin + 2) * kTileP, true, f_limit(it_begin + 2));
+      if constexpr (kBoth) {
+        Fp4Regs k0 = fp4_issue(p0, false), v0 = fp4_issue(p0, true), k1 = fp4_issue(p1, false);
+        f_k = fp4_issue(f_ahead, false);
+        f_v = fp4_issue(p1, true);
+        fp4_stage(k0, klds(0), false);
+        fp4_stage(v0, vlds(0), true);
+        fp4_stage(k1, klds(1), false);
+      } else if (f_role == 0) {
+        Fp4Regs k0 = fp4_issue(p0, false), k1 = fp4_issue(p1, false);
+        f_k = fp4_issue(f_ahead, false);
+        fp4_stage(k0, klds(0), false);
+        fp4_stage(k1, klds(1), false);
+      } else if (f_role == 1) {
+        Fp4Regs v0 = fp4_issue(p0, true);
+        f_k = fp4_issue(p1, true);
+        fp4_stage(v0, vlds(0), true);
+      }
+      page_chunk = chunk_of((it_begin + (f_role == 0 ? 3 : 2)) * kTileP);
+      page_ids = load_page_ids(page_chunk);
+      __syncthreads();
+    } else
     if constexpr (kDirect) {
       ahead = find_pages(it_begin * kTileP, true, kv_len);
       dma_keys(ahead, klds(0));
@@ -992,7 +1127,20 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
   // scores and its first half's weights.
   auto step = [&](int it, int buf) {
     TilePages value_pages{};
-    if constexpr (kDirect) {
+    Fp4Pages f_pages{};
+    if constexpr (kFp4) {
+      __syncthreads();
+      if constexpr (kBoth) {
+        f_pages = f_ahead;
+        f_ahead = fp4_find((it + 3) * kTileP, false, f_limit(it + 3));
+        fp4_turn(f_v, true);
+        fp4_turn(f_k, false);
+      } else if (f_role < 2) {
+        const int next = f_role == 0 ? it + 3 : it + 2;
+        f_ahead = fp4_find(next * kTileP, false, f_limit(next));
+        fp4_turn(f_k, f_role == 1);
+      }
+    } else if constexpr (kDirect) {
       __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
       __syncthreads();
       value_pages = ahead;
@@ -1006,13 +1154,27 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
     auto load_value = [&](int j) {
       if constexpr (kDirect) {
         if (j < NI) dma_value(value_pages, vlds(buf ^ 1), j);
+      } else if constexpr (kFp4 && kBoth) {
+        if (j < 4) fp4_put(f_v, vlds(buf ^ 1), true, j);
+        if (j == 3) f_v = fp4_issue(f_pages, true);
       }
     };
     auto load_key = [&](int j) {
       if constexpr (kDirect) {
         if (j < NI) dma_key(ahead, klds(buf), j);
+      } else if constexpr (kFp4 && kBoth) {
+        if (j < 4) fp4_put(f_k, klds(buf), false, j);
+        if (j == 3) f_k = fp4_issue(f_ahead, false);
       }
     };
+    if constexpr (kFp4 && !kBoth) {
+      if (f_role < 2) {  // uniform
+        uint16_t* const dst = f_role == 0 ? klds(buf) : vlds(buf ^ 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fp4_put(f_k, dst, f_role == 1, j);
+        f_k = fp4_issue(f_ahead, f_role == 1);
+      }
+    }
     if (wave_live) {
       mask(s_odd, it * kTileP + 32);
       half_step(buf ^ 1, 0, s_even, buf, 0, pb_even, s_odd, true, pb_odd, load_value);
@@ -1021,6 +1183,12 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
     } else if constexpr (kDirect) {
       dma_values(value_pages, vlds(buf ^ 1));
       dma_keys(ahead, klds(buf));
+    } else if constexpr (kFp4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        load_value(j);
+        load_key(j);
+      }
     }
   };
   auto last_step = [&](int it, int buf) {
@@ -1542,7 +1710,21 @@ int64_t context_partial_bytes(int64_t rows, int64_t row_tokens, int64_t num_q_he
 
 template <int kWork>
 void launch_context(int64_t head_dim, int waves, int mode, dim3 grid, dim3 block, hipStream_t stream,
-                    const ContextArgs& a) {
+                    const ContextArgs& a, const Fp4Cache* fp4) {
+  if (fp4 != nullptr) {
+    Fp4ContextArgs f{};
+    static_cast<ContextArgs&>(f) = a;
+    f.c = *fp4;
+    if (head_dim == 64 && waves == 8)
+      hipLaunchKernelGGL((context_attn<64, kPagesFp4, 8, kWork>), grid, block, 0, stream, f);
+    else if (head_dim == 64)
+      hipLaunchKernelGGL((context_attn<64, kPagesFp4, 4, kWork>), grid, block, 0, stream, f);
+    else if (waves == 8)
+      hipLaunchKernelGGL((context_attn<128, kPagesFp4, 8, kWork>), grid, block, 0, stream, f);
+    else
+      hipLaunchKernelGGL((context_attn<128, kPagesFp4, 4, kWork>), grid, block, 0, stream, f);
+    return;
+  }
   if (head_dim == 64) {
     if (waves == 8) launch_context_mode<64, 8, kWork>(mode, grid, block, stream, a);
     else launch_context_mode<64, 4, kWork>(mode, grid, block, stream, a);
@@ -1569,21 +1751,16 @@ PlanLayout plan_layout(int64_t units_bound, int64_t head_blocks, int64_t residen
   return {item_cap, units_bound, 256 + 32 * item_cap + 32 * units_bound};
 }
 
-}  // namespace
-}  // namespace mas
-
-extern "C" int mas_paged_context_attention_bf16(void* out, int64_t out_stride, int64_t out_head_stride, const void* q,
-                                                int64_t q_stride, int64_t q_head_stride, const void* k_cache,
-                                                const void* v_cache, int64_t page_stride, int64_t entry_stride,
-                                                int64_t head_stride, int64_t num_pages, int64_t page_size,
-                                                const int32_t* block_tables, int64_t block_table_stride,
-                                                int64_t max_blocks, const int32_t* seq_lens,
-                                                const int32_t* cu_seqlens_q, int64_t num_rows, int64_t max_q_len,
-                                                int64_t max_kv_len, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
-                                                float bmm1_scale, float bmm2_scale, int out_fp8,
-                                                const float* out_scale_dev, float out_scale_host, void* workspace,
-                                                int64_t workspace_bytes, uint32_t* err, hipStream_t stream) {
-  using namespace mas;
+// The call over either cache: `fp4` null for the bf16 one (k_cache, v_cache and their strides).
+int context_attention(void* out, int64_t out_stride, int64_t out_head_stride, const void* q, int64_t q_stride,
+                      int64_t q_head_stride, const void* k_cache, const void* v_cache, int64_t page_stride,
+                      int64_t entry_stride, int64_t head_stride, const Fp4Cache* fp4, int64_t num_pages,
+                      int64_t page_size, const int32_t* block_tables, int64_t block_table_stride, int64_t max_blocks,
+                      const int32_t* seq_lens, const int32_t* cu_seqlens_q, int64_t num_rows, int64_t max_q_len,
+                      int64_t max_kv_len, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                      float bmm1_scale, float bmm2_scale, int out_fp8, const float* out_scale_dev,
+                      float out_scale_host, void* workspace, int64_t workspace_bytes, uint32_t* err,
+                      hipStream_t stream) {
   if (num_rows < 0 || max_q_len < 0 || num_q_heads < 0 || num_kv_heads < 0 || num_pages < 0 || page_size <= 0 ||
       max_blocks < 0 || workspace_bytes < 0)
     return MAS_ERR_INVALID_VALUE;
@@ -1594,13 +1771,16 @@ extern "C" int mas_paged_context_attention_bf16(void* out, int64_t out_stride, i
   if ((head_dim != 64 && head_dim != 128) || (page_size & (page_size - 1)) != 0) return MAS_ERR_UNSUPPORTED;
   const int64_t cap = max_blocks * page_size;
   if (cap > (int64_t{1} << 30) || num_rows > 65535 || num_q_heads > 65535) return MAS_ERR_UNSUPPORTED;
-  if (out == nullptr || q == nullptr || seq_lens == nullptr || cu_seqlens_q == nullptr || k_cache == nullptr ||
-      v_cache == nullptr || block_tables == nullptr || num_pages == 0 || cap == 0)
+  if (out == nullptr || q == nullptr || seq_lens == nullptr || cu_seqlens_q == nullptr ||
+      (fp4 == nullptr && (k_cache == nullptr || v_cache == nullptr)) || block_tables == nullptr || num_pages == 0 ||
+      cap == 0)
     return MAS_ERR_INVALID_VALUE;
-  const bool aligned = aligned16(q) && aligned16(out) && aligned16(k_cache) && aligned16(v_cache) &&
-                       q_stride % 8 == 0 && q_head_stride % 8 == 0 && out_stride % 8 == 0 &&
-                       out_head_stride % 8 == 0 && page_stride % 8 == 0 && entry_stride % 8 == 0 &&
-                       head_stride % 8 == 0;
+  // (check_fp4_cache saw to the 4-bit cache's own; its in-page byte offsets are 32-bit numbers)
+  if (fp4 != nullptr && (fp4->entry_stride < 0 || page_size * fp4->entry_stride > INT32_MAX)) return MAS_ERR_UNSUPPORTED;
+  const bool aligned = aligned16(q) && aligned16(out) && q_stride % 8 == 0 && q_head_stride % 8 == 0 &&
+                       out_stride % 8 == 0 && out_head_stride % 8 == 0 &&
+                       (fp4 != nullptr || (aligned16(k_cache) && aligned16(v_cache) && page_stride % 8 == 0 &&
+                                           entry_stride % 8 == 0 && head_stride % 8 == 0));
   if (!aligned) return MAS_ERR_MISALIGNED;
   const int64_t group = num_q_heads / num_kv_heads;
   const ContextLaunch shape = context_launch(group);
@@ -1744,7 +1924,7 @@ extern "C" int mas_paged_context_attention_bf16(void* out, int64_t out_stride, i
     a.plan_cap = cap;
     a.part_o = reinterpret_cast<float*>(ws + self_plan_partial_off(units_bound));
     a.part_ml = a.part_o + plan_entries * head_dim;
-    launch_context<kWorkSelfPlan>(head_dim, waves, mode, dim3(static_cast<uint32_t>(plan.item_cap)), block, stream, a);
+    launch_context<kWorkSelfPlan>(head_dim, waves, mode, dim3(static_cast<uint32_t>(plan.item_cap)), block, stream, a, fp4);
     if (const int st = launch_status(); st != MAS_OK) return st;
   } else if (planned) {
     uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1776,7 +1956,7 @@ extern "C" int mas_paged_context_attention_bf16(void* out, int64_t out_stride, i
     a.part_ml = a.part_o + plan_entries * head_dim;
     hipLaunchKernelGGL(context_plan, dim3(1), dim3(kPlanThreads), 0, stream, pa);
     if (const int st = launch_status(); st != MAS_OK) return st;
-    launch_context<kWorkPlan>(head_dim, waves, mode, dim3(static_cast<uint32_t>(plan.item_cap)), block, stream, a);
+    launch_context<kWorkPlan>(head_dim, waves, mode, dim3(static_cast<uint32_t>(plan.item_cap)), block, stream, a, fp4);
     if (const int st = launch_status(); st != MAS_OK) return st;
   }
   if (planned) {
@@ -1794,7 +1974,7 @@ extern "C" int mas_paged_context_attention_bf16(void* out, int64_t out_stride, i
   }
   if (kv_splits > 1) {
     const dim3 grid(static_cast<uint32_t>(gx), static_cast<uint32_t>(gy), static_cast<uint32_t>(num_rows * kv_splits));
-    launch_context<kWorkSplit>(head_dim, waves, mode, grid, block, stream, a);
+    launch_context<kWorkSplit>(head_dim, waves, mode, grid, block, stream, a, fp4);
   } else {
     // Rows in turn (their tiles longest first) keep a row's key / value tiles warm in L2 while its
     // workgroups run, but the last row's longest tiles then start late: the launch ends on them.
@@ -1820,7 +2000,7 @@ extern "C" int mas_paged_context_attention_bf16(void* out, int64_t out_stride, i
     const dim3 grid = a.tile_major
                           ? dim3(static_cast<uint32_t>(gx), static_cast<uint32_t>(num_rows), static_cast<uint32_t>(gy))
                           : dim3(static_cast<uint32_t>(gx), static_cast<uint32_t>(gy), static_cast<uint32_t>(num_rows));
-    launch_context<kWorkGrid>(head_dim, waves, mode, grid, block, stream, a);
+    launch_context<kWorkGrid>(head_dim, waves, mode, grid, block, stream, a, fp4);
   }
   if (const int st = launch_status(); st != MAS_OK || kv_splits == 1) return st;
   const int64_t merges = num_rows * row_tokens * num_q_heads;  // <= INT32_MAX when split
@@ -1831,6 +2011,59 @@ extern "C" int mas_paged_context_attention_bf16(void* out, int64_t out_stride, i
     hipLaunchKernelGGL(context_combine<128>, dim3(static_cast<uint32_t>(merges)), dim3(64), 0, stream, a,
                        static_cast<int>(tokens_per_wg));
   return launch_status();
+}
+
+}  // namespace
+}  // namespace mas
+
+extern "C" int mas_paged_context_attention_bf16(void* out, int64_t out_stride, int64_t out_head_stride, const void* q,
+                                                int64_t q_stride, int64_t q_head_stride, const void* k_cache,
+                                                const void* v_cache, int64_t page_stride, int64_t entry_stride,
+                                                int64_t head_stride, int64_t num_pages, int64_t page_size,
+                                                const int32_t* block_tables, int64_t block_table_stride,
+                                                int64_t max_blocks, const int32_t* seq_lens,
+                                                const int32_t* cu_seqlens_q, int64_t num_rows, int64_t max_q_len,
+                                                int64_t max_kv_len, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                                float bmm1_scale, float bmm2_scale, int out_fp8,
+                                                const float* out_scale_dev, float out_scale_host, void* workspace,
+                                                int64_t workspace_bytes, uint32_t* err, hipStream_t stream) {
+  return mas::context_attention(out, out_stride, out_head_stride, q, q_stride, q_head_stride, k_cache, v_cache,
+                                page_stride, entry_stride, head_stride, nullptr, num_pages, page_size, block_tables,
+                                block_table_stride, max_blocks, seq_lens, cu_seqlens_q, num_rows, max_q_len,
+                                max_kv_len, num_q_heads, num_kv_heads, head_dim, bmm1_scale, bmm2_scale, out_fp8,
+                                out_scale_dev, out_scale_host, workspace, workspace_bytes, err, stream);
+}
+
+extern "C" int mas_paged_context_attention_fp4(void* out, int64_t out_stride, int64_t out_head_stride, const void* q,
+                                               int64_t q_stride, int64_t q_head_stride, const void* k_cache,
+                                               const void* v_cache, int64_t page_stride, int64_t entry_stride,
+                                               int64_t head_stride, const void* k_scale, const void* v_scale,
+                                               int64_t scale_page_stride, int64_t scale_head_stride, int64_t num_pages,
+                                               int64_t page_size, const int32_t* block_tables,
+                                               int64_t block_table_stride, int64_t max_blocks, const int32_t* seq_lens,
+                                               const int32_t* cu_seqlens_q, int64_t num_rows, int64_t max_q_len,
+                                               int64_t max_kv_len, int64_t num_q_heads, int64_t num_kv_heads,
+                                               int64_t head_dim, float bmm1_scale, float bmm2_scale, int out_fp8,
+                                               const float* out_scale_dev, float out_scale_host, void* workspace,
+                                               int64_t workspace_bytes, uint32_t* err, hipStream_t stream) {
+  using namespace mas;
+  Fp4Cache c{};
+  c.k = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  c.v = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  c.page_stride = page_stride;
+  c.entry_stride = entry_stride;
+  c.head_stride = head_stride;
+  c.k_scale = static_cast<uint8_t*>(const_cast<void*>(k_scale));
+  c.v_scale = static_cast<uint8_t*>(const_cast<void*>(v_scale));
+  c.scale_page_stride = scale_page_stride;
+  c.scale_head_stride = scale_head_stride;
+  c.num_pages = num_pages;
+  c.page_size = page_size;
+  if (const int st = check_fp4_cache(c); st != MAS_OK) return st;
+  return context_attention(out, out_stride, out_head_stride, q, q_stride, q_head_stride, nullptr, nullptr, 0, 0, 0, &c,
+                           num_pages, page_size, block_tables, block_table_stride, max_blocks, seq_lens, cu_seqlens_q,
+                           num_rows, max_q_len, max_kv_len, num_q_heads, num_kv_heads, head_dim, bmm1_scale,
+                           bmm2_scale, out_fp8, out_scale_dev, out_scale_host, workspace, workspace_bytes, err, stream);
 }
 
 extern "C" int64_t mas_paged_context_attention_workspace_bytes(int64_t num_rows, int64_t max_q_len,

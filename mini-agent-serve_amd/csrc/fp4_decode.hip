@@ -1,0 +1,401 @@
+// fp4_decode.hip - paged decode attention over the 4-bit KV cache that fp4_cache.hip writes.
+//
+// For decode row b and query head h (kv head h / G, G = Hq / Hk), over the positions p < seq_lens[b], whose
+// codes and powers (fp4.h) sit at page = block_tables[b, p / page_size], entry = p % page_size:
+//   s_p = bmm1_scale * (q[b, h] . k_p),   out[b, h] = bmm2_scale * sum_p softmax(s)_p * v_p,
+// k_p and v_p the values the codes stand for; fp32 sums, rounded once to bf16 (decode attention over the
+// bf16 cache, devstral2.py:184-196, on another cache format).
+//
+// Split-KV as there (decode_split.h): a wavefront per (kv head, split, row), then the merge of the splits.
+// A split is walked in steps of 32 positions, two 16-position tiles, entirely in registers:
+//   S^T = K Q^T on v_mfma_f32_16x16x32_bf16: lane (n, r) loads quarter r of key row n (32 codes of head_dim 128, one
+//     block) and decodes it (v_cvt_scalef32_pk_bf16_fp4, exact); the columns of B are the kv head's query heads, with
+//     the head dim numbered as the lanes hold it. (The scaled MFMAs take e2m1 operands as they lie in memory, but
+//     sum groups of 8 products in a window of 14 bits below the largest - checked on MI355X - where the bf16 ones keep
+//     24: with queries as two e4m3 terms, scores of large terms were off by up to 2^-10 of them.)
+//   P^T = softmax weights in the result's layout: lane (n, r) holds head n at positions 4 r + j of both
+//     tiles, which is the layout of the B operand of the next product when its 32 positions are numbered that way.
+//   O^T += V^T P^T on v_mfma_f32_16x16x32_bf16: lane (n, r) reads, for its 8 positions, the D / 16 codes of
+//     head-dim elements D / 16 * n .. and decodes them; a byte permute per word pairs positions instead of elements. P enters as two bf16 terms, so it keeps 16 significant bits.
+// The softmax's reference m is lazy: a step's weights are taken against the m the row has, and only where a
+// lane's sum over the step passes 2^8 (or is NaN or infinite: the first step's m is -inf) does m move to the maximum.
+// What bounds it: HBM for long rows (68 bytes per head and position at head_dim 128, each of keys and values),
+// launch and memory latency for few.
+#include "decode_split.h"
+#include "fp4.h"
+
+namespace mas {
+namespace {
+
+constexpr float kSumMost = 256.f;
+
+struct Fp4DecodeArgs : DecodeArgs {
+  Fp4Cache c;
+};
+
+// One step's keys and values as they lie in the cache.
+template <int D>
+struct Fp4Loads {
+  static constexpr int KW = D / 32;                       // words of a lane's quarter of a key row
+  static constexpr int KP = D == 256 ? 2 : 1;             // powers of it
+  static constexpr int VW = D / 128 > 0 ? D / 128 : 1;    // words of value codes per position (64: half a word)
+  uint32_t k[2][KW];
+  uint32_t ks[2][KP];
+  uint32_t v[2][4][VW];
+  uint32_t vs[2];
+  int count[2];  // valid positions of each tile (wavefront-uniform)
+};
+
+template <int D, int kHeads>
+__global__ __launch_bounds__(64 * kHeads, D <= 128 ? 3 : 1) void fp4_decode_split(Fp4DecodeArgs a) {
+  using Loads = Fp4Loads<D>;
+  constexpr int EL = D / 16;     // head-dim elements per lane of the value operand: EL n ..
+  constexpr int NB = EL / 2;     // their code bytes per position
+  constexpr int kStep = 32;
+  const int lane = threadIdx.x & 63;
+  const int wave = wave_id_uniform();
+  const int kvh = blockIdx.x * kHeads + wave;
+  const int b = blockIdx.z;
+  // the splits of row b rotated over the grid, as in the bf16 kernel: rows shorter than the table have only
+  // their first splits to do, which would all land on the same XCDs
+  const unsigned turn = gridDim.y & 1 ? 0u : blockIdx.z + (blockIdx.z >> 2);
+  const int split = static_cast<int>((blockIdx.y + turn) % gridDim.y);
+  const int L = kv_len(a, b);
+  const int split_len = row_split_len(a, L);
+  const int start = split * split_len;
+  if (start >= L) return;
+  const int end = min(start + split_len, L);
+  const int G = a.group;
+  const int n = lane & 15, r = lane >> 4;
+
+  // Block-table entries of the split: lane i holds entry first + i.
+  const int32_t* bt = a.block_tables + b * a.bt_stride;
+  int first = start >> a.log2_page;
+  auto load_entries = [&] { return bt[min(static_cast<int64_t>(first + lane), a.max_blocks - 1)]; };
+  int entries = load_entries();
+  // B operands of S^T = K Q^T: head n, head-dim elements D / 4 r + 8 j + 0..7 (zeros past the group)
+  constexpr int KJ = D / 32;
+  bf16x8 q[KJ];
+  {
+    const uint16_t* row = a.q + b * a.q_stride + static_cast<int64_t>(kvh * G + (n < G ? n : 0)) * a.q_head_stride;
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+      u32x4 v = load_cached(row + D / 4 * r + 8 * j);
+      if (n >= G) v = u32x4{0u, 0u, 0u, 0u};
+      q[j] = __builtin_bit_cast(bf16x8, v);
+    }
+  }
+
+  const uint32_t es = static_cast<uint32_t>(a.c.entry_stride), ps = static_cast<uint32_t>(a.c.page_size);
+  // this lane's byte offsets in a tile: its quarter of its key row, its value rows' codes, and their powers
+  const uint32_t k_off = n * es + D / 8 * r;
+  const uint32_t ks_off = (D / 4 * r / kFp4Block) * ps + n;
+  const uint32_t v_off = 4 * r * es + n * NB;
+  const uint32_t vs_off = (n * EL / kFp4Block) * ps + 4 * r;
+  const int mask = static_cast<int>(a.c.page_size) - 1;
+  const uint8_t* const k_head = a.c.k + kvh * a.c.head_stride;
+  const uint8_t* const v_head = a.c.v + kvh * a.c.head_stride;
+  const uint8_t* const ks_head = a.c.k_scale + kvh * a.c.scale_head_stride;
+  const uint8_t* const vs_head = a.c.v_scale + kvh * a.c.scale_head_stride;
+
+  bool bad = false;
+  auto issue = [&](Loads& st, int pos) {
+    int64_t at[2], sat[2];  // byte offsets of the tiles' first rows and powers
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int p = pos + 16 * t;
+      const int pc = p < end ? p : end - 1;  // a tile past the end reads the last position's page
+      const int entry = pc >> a.log2_page;
+      if (entry - first >= 64) {  // uniform
+        first = entry;
+        entries = load_entries();
+      }
+      const int32_t page = __builtin_amdgcn_readlane(entries, entry - first);
+      const bool ok = page >= 0 && page < a.c.num_pages;
+      st.count[t] = ok ? max(0, min(16, end - p)) : 0;
+      bad |= !ok;
+      const int64_t pg = ok ? page : 0;
+      const uint32_t slot = static_cast<uint32_t>(pc & mask & ~15);
+      at[t] = pg * a.c.page_stride + static_cast<int64_t>(slot) * es;
+      sat[t] = pg * a.c.scale_page_stride + slot;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* src = k_head + at[t] + k_off;
+      if constexpr (D == 64) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+        st.k[t][0] = x[0];
+        st.k[t][1] = x[1];
+      } else {
+#pragma unroll
+        for (int h = 0; h < D / 128; ++h) {
+          const u32x4 x = load_cached(src + 16 * h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.k[t][4 * h + i] = x[i];
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < Loads::KP; ++h) st.ks[t][h] = (ks_head + sat[t])[ks_off + h * ps];
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* base = v_head + at[t];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* src = base + static_cast<int64_t>(i) * es + v_off;
+        if constexpr (D == 64) {
+          st.v[t][i][0] = *reinterpret_cast<const uint16_t*>(src);
+        } else if constexpr (D == 128) {
+          st.v[t][i][0] = *reinterpret_cast<const uint32_t*>(src);
+        } else {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+          st.v[t][i][0] = x[0];
+          st.v[t][i][1] = x[1];
+        }
+      }
+      st.vs[t] = *reinterpret_cast<const uint32_t*>(vs_head + sat[t] + vs_off);
+    }
+  };
+
+  float m_run = kNegInf, l_run = 0.f;  // head n's reference (in all four lanes), this lane's share of its sum
+  f32x4 acc[EL];  // O^T: element j of acc[e] holds O[head n][EL (4 r + j) + e]
+#pragma unroll
+  for (int e = 0; e < EL; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](Loads& st) {
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) {
+        const float f = __uint_as_float(st.ks[t][j * Loads::KP / KJ] << 23);
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fp4x8_decode(st.k[t][j], f)), q[j],
+                                                       s[t], 0, 0, 0);
+      }
+      s[t] *= a.scale_log2;
+      if (st.count[t] < 16) {  // uniform: the row's end, or a page outside the cache
+        const int left = st.count[t] - 4 * r;  // valid positions of this lane's four
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j >= left) {
+            s[t][j] = kNegInf;
+#pragma unroll
+            for (int x = 0; x < Loads::VW; ++x) st.v[t][j][x] = 0u;
+          }
+        st.vs[t] = left >= 4 ? st.vs[t] : left <= 0 ? 0u : st.vs[t] & ((1u << (8 * left)) - 1u);
+      }
+    }
+    float p[8], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - m_run);
+      sum += p[e];
+    }
+    const uint64_t over = __builtin_amdgcn_ballot_w64(!(sum <= kSumMost));
+    if (over != 0) {  // some head's reference moves
+      const uint32_t heads = static_cast<uint32_t>(over | over >> 16 | over >> 32 | over >> 48) & 0xffffu;
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const bool moves = (heads >> n) & 1u;
+      const float m_new = moves ? fmaxf(m_run, mx) : m_run;
+      const float alpha = moves && m_run != kNegInf ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int e = 0; e < EL; ++e) acc[e] *= alpha;
+      const float m_use = m_run == kNegInf ? 0.f : m_run;
+      sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - m_use);
+        sum += p[e];
+      }
+    }
+    l_run += sum;
+    u32x4 ph, pl;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      ph[e] = pack_bf16x2(p[2 * e], p[2 * e + 1]);
+      pl[e] = pack_bf16x2(p[2 * e] - bf16_lo(ph[e]), p[2 * e + 1] - bf16_hi(ph[e]));
+    }
+    const bf16x8 p_hi = __builtin_bit_cast(bf16x8, ph), p_lo = __builtin_bit_cast(bf16x8, pl);
+    float f[2][4];  // the positions' powers, as the decode's scales
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f[t][0] = __uint_as_float(st.vs[t] << 23);
+      f[t][1] = __uint_as_float(st.vs[t] << 15);
+      f[t][2] = __uint_as_float(st.vs[t] << 7);
+      f[t][3] = __uint_as_float(st.vs[t] >> 1);
+    }
+    auto weigh = [&](auto byte) {
+      constexpr int c = decltype(byte)::value;
+      u32x4 even, odd;  // elements 2 c and 2 c + 1 of this lane at its 8 positions
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t x = fp4x2_decode<c & 3>(st.v[t][2 * i][c >> 2], f[t][2 * i]);
+          const uint32_t y = fp4x2_decode<c & 3>(st.v[t][2 * i + 1][c >> 2], f[t][2 * i + 1]);
+          even[2 * t + i] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+          odd[2 * t + i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+        }
+      const bf16x8 ve = __builtin_bit_cast(bf16x8, even), vo = __builtin_bit_cast(bf16x8, odd);
+      acc[2 * c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, p_lo, acc[2 * c], 0, 0, 0);
+      acc[2 * c + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, p_lo, acc[2 * c + 1], 0, 0, 0);
+      acc[2 * c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, p_hi, acc[2 * c], 0, 0, 0);
+      acc[2 * c + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, p_hi, acc[2 * c + 1], 0, 0, 0);
+    };
+    weigh(std::integral_constant<int, 0>{});
+    weigh(std::integral_constant<int, 1>{});
+    if constexpr (NB > 2) {
+      weigh(std::integral_constant<int, 2>{});
+      weigh(std::integral_constant<int, 3>{});
+    }
+    if constexpr (NB > 4) {
+      weigh(std::integral_constant<int, 4>{});
+      weigh(std::integral_constant<int, 5>{});
+      weigh(std::integral_constant<int, 6>{});
+      weigh(std::integral_constant<int, 7>{});
+    }
+  };
+
+  // Two load buffers used in turn: a step is computed while the next one's loads are in flight.
+  const int nsteps = (end - start + kStep - 1) / kStep;
+  Loads ld0, ld1;
+  issue(ld0, start);
+  int i = 0;
+  for (; i + 2 < nsteps; i += 2) {
+    issue(ld1, start + (i + 1) * kStep);
+    compute(ld0);
+    issue(ld0, start + (i + 2) * kStep);
+    compute(ld1);
+  }
+  if (i + 1 < nsteps) {
+    issue(ld1, start + (i + 1) * kStep);
+    compute(ld0);
+    compute(ld1);
+  } else {
+    compute(ld0);
+  }
+  if (__builtin_amdgcn_ballot_w64(bad) != 0 && lane == 0) report(a.err, MAS_ERRBIT_PAGE);
+
+  l_run += __shfl_xor(l_run, 16);
+  l_run += __shfl_xor(l_run, 32);
+  if (n >= G) return;
+  const int h = kvh * G + n;
+  if (L <= split_len) {  // the row's only split: its output
+    const float sc = l_run > 0.f ? a.out_scale / l_run : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < EL; e += 4) {
+        const float y[4] = {acc[e][j] * sc, acc[e + 1][j] * sc, acc[e + 2][j] * sc, acc[e + 3][j] * sc};
+        store_output<4>(a, b, h, EL * (4 * r + j) + e, y);
+      }
+    return;
+  }
+  const int64_t at = (static_cast<int64_t>(b) * a.hq + h) * a.max_splits + split;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < EL; e += 4)
+      __builtin_nontemporal_store(f32x4{acc[e][j], acc[e + 1][j], acc[e + 2][j], acc[e + 3][j]},
+                                  reinterpret_cast<f32x4*>(a.part_o + at * D + EL * (4 * r + j) + e));
+  if (r == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m_run, l_run};
+}
+
+template <int D>
+int launch_fp4_decode(const Fp4DecodeArgs& a, int64_t batch, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>(a.hk), static_cast<uint32_t>(a.max_splits), static_cast<uint32_t>(batch));
+  hipLaunchKernelGGL((fp4_decode_split<D, 1>), grid, dim3(64), 0, s, a);
+  if (const int st = launch_status(); st != MAS_OK) return st;
+  hipLaunchKernelGGL((decode_attn_combine<D>), dim3(static_cast<uint32_t>(a.hq), static_cast<uint32_t>(batch)),
+                     dim3(64), 0, s, a);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace mas
+
+extern "C" int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int64_t out_head_stride, const void* q,
+                                              int64_t q_stride, int64_t q_head_stride, const void* k_cache,
+                                              const void* v_cache, int64_t page_stride, int64_t entry_stride,
+                                              int64_t head_stride, const void* k_scale, const void* v_scale,
+                                              int64_t scale_page_stride, int64_t scale_head_stride, int64_t num_pages,
+                                              int64_t page_size, const int32_t* block_tables,
+                                              int64_t block_table_stride, int64_t max_blocks, const int32_t* seq_lens,
+                                              int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                              int64_t head_dim, float bmm1_scale, float bmm2_scale, int out_fp8,
+                                              const float* out_scale_dev, float out_scale_host, void* workspace,
+                                              int64_t workspace_bytes, uint32_t* err, hipStream_t stream) {
+  using namespace mas;
+  if (batch < 0 || num_q_heads < 0 || num_kv_heads < 0 || max_blocks < 0 || workspace_bytes < 0)
+    return MAS_ERR_INVALID_VALUE;
+  Fp4DecodeArgs a{};
+  a.c.k = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  a.c.v = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  a.c.page_stride = page_stride;
+  a.c.entry_stride = entry_stride;
+  a.c.head_stride = head_stride;
+  a.c.k_scale = static_cast<uint8_t*>(const_cast<void*>(k_scale));
+  a.c.v_scale = static_cast<uint8_t*>(const_cast<void*>(v_scale));
+  a.c.scale_page_stride = scale_page_stride;
+  a.c.scale_head_stride = scale_head_stride;
+  a.c.num_pages = num_pages;
+  a.c.page_size = page_size;
+  if (const int st = check_fp4_cache(a.c); st != MAS_OK) return st;
+  if (batch == 0 || num_q_heads == 0) return MAS_OK;
+  if (num_kv_heads == 0 || num_q_heads % num_kv_heads != 0) return MAS_ERR_INVALID_VALUE;
+  const int64_t group = num_q_heads / num_kv_heads;
+  if (group > 16 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return MAS_ERR_UNSUPPORTED;
+  const int64_t cap = max_blocks * page_size;
+  // (a page's rows are addressed with 32-bit byte offsets)
+  if (cap > (int64_t{1} << 30) || batch > 65535 || num_kv_heads > 65535 || num_q_heads > 65535 || entry_stride < 0 ||
+      page_size * entry_stride > INT32_MAX)
+    return MAS_ERR_UNSUPPORTED;
+  if (out == nullptr || q == nullptr || seq_lens == nullptr ||
+      (cap > 0 && (block_tables == nullptr || num_pages == 0)))
+    return MAS_ERR_INVALID_VALUE;
+  if (out_fp8 && out_scale_dev == nullptr && !(out_scale_host > 0.f)) return MAS_ERR_INVALID_VALUE;
+  if (!aligned16(q) || !aligned16(out) || q_stride % 8 != 0 || q_head_stride % 8 != 0 || out_stride % 8 != 0 ||
+      out_head_stride % 8 != 0 || !aligned16(workspace))
+    return MAS_ERR_MISALIGNED;
+  DecodeSplits sp{};
+  if (const int st = decode_splits(batch, num_q_heads, num_kv_heads, head_dim, cap, workspace, workspace_bytes, &sp);
+      st != MAS_OK)
+    return st == kWorkspaceTooSmall ? MAS_ERR_INVALID_VALUE : st;
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_stride = q_stride;
+  a.q_head_stride = q_head_stride;
+  a.num_pages = num_pages;
+  a.block_tables = block_tables;
+  a.bt_stride = block_table_stride;
+  a.max_blocks = max_blocks;
+  a.seq_lens = seq_lens;
+  a.hq = static_cast<int>(num_q_heads);
+  a.hk = static_cast<int>(num_kv_heads);
+  a.group = static_cast<int>(group);
+  while ((int64_t{1} << a.log2_page) < page_size) ++a.log2_page;
+  a.split_len = static_cast<int>(sp.split_len);
+  a.row_target = sp.row_target;
+  a.max_splits = static_cast<int>(sp.splits);
+  a.scale_log2 = bmm1_scale * 1.4426950408889634f;
+  a.out_scale = bmm2_scale;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + batch * num_q_heads * sp.splits * head_dim;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.out_head_stride = out_head_stride;
+  a.out_fp8 = out_fp8 != 0;
+  a.quant_scale_dev = out_scale_dev;
+  a.quant_scale_host = out_scale_host;
+  a.err = err;
+  switch (head_dim) {
+    case 64: return launch_fp4_decode<64>(a, batch, stream);
+    case 128: return launch_fp4_decode<128>(a, batch, stream);
+    default: return launch_fp4_decode<256>(a, batch, stream);
+  }
+}

@@ -1,0 +1,199 @@
+// step_plan.hip - a step's index tensors from its rows' lengths, on the device.
+//
+// What the reference's runner fills on the host for every step (ModelRunner.prepare,
+// miniagentserve/engine/model_runner.py:176-225) and its block manager hands it pages for
+// (miniagentserve/engine/block_manager.py:43-73). Row r holds c_r positions and gets n_r new tokens, rows in order:
+//   cu_seqlens_q[r + 1] = sum of n_0 .. n_r,  seq_lens[r] = c_r + n_r;
+//   token t of row r (cu[r] <= t < cu[r + 1]): position p = c_r + t - cu[r], batch index r,
+//     slot = page * page_size + p % page_size with page = block_tables[r, p / page_size];
+//   the pages of blocks ceil(c_r / page_size) .. ceil((c_r + n_r) / page_size) - 1 are taken from the free ring
+//     in row order and written to the row's block table.
+// Rows are served as long as the free pages and the token count reach: from the first row that does not fit
+// on, rows get no token (MAS_ERRBIT_POOL). A row with a negative length or one past its table is passed over
+// (MAS_ERRBIT_POSITION).
+//
+// One thread per token, and every workgroup sums the rows' tokens and pages itself, 256 rows at a time (a row
+// per thread, both sums in one pass of wavefront scans), until its own tokens are covered: no workgroup
+// waits for another, and one launch does it. What bounds it: the latencies of the lengths, the page and the stores.
+#include "device.h"
+
+namespace mas {
+namespace {
+
+constexpr int kPlanBlock = 256;
+constexpr int kPlanWaves = kPlanBlock / kWave;
+
+struct StepArgs {
+  int32_t* positions;
+  int32_t* batch_indices;
+  int64_t* slots;
+  int32_t* cu;
+  int32_t* seq_lens;
+  int64_t* range_out;
+  int32_t* tables;
+  int64_t bt_stride, max_blocks;
+  const int32_t* new_lens;
+  const int32_t* cached_lens;
+  int64_t rows;
+  const int32_t* free_pages;
+  int64_t ring;
+  const int64_t* range;
+  int64_t page_size, num_tokens;
+  uint32_t* err;
+};
+
+__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int64_t o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+__device__ __forceinline__ int64_t wave_max64(int64_t v) {
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d /= 2) v = max(v, static_cast<int64_t>(__shfl_xor(v, d)));
+  return v;
+}
+
+__global__ __launch_bounds__(kPlanBlock) void plan_step(StepArgs a) {
+  __shared__ int64_t sums[2][kPlanWaves], tops[2][kPlanWaves];
+  __shared__ int ends[kPlanBlock];                       // token past the row's last one
+  __shared__ int row_new[kPlanBlock], row_cached[kPlanBlock], row_page[kPlanBlock];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kPlanBlock + tid;
+  const int64_t last_t = min(static_cast<int64_t>(blockIdx.x + 1) * kPlanBlock, a.num_tokens);
+  const bool writer = blockIdx.x == 0;  // of the rows' outputs
+  const int64_t head = a.range[0], tail = a.range[1];
+  const int64_t avail = head < 0 || tail < head ? 0 : min(tail - head, a.ring);
+  const int64_t head_at = a.ring > 0 && head >= 0 ? head % a.ring : 0;
+  const int64_t reach = a.max_blocks * a.page_size;
+  const uint32_t ps = static_cast<uint32_t>(a.page_size);
+
+  int64_t tokens = 0, pages = 0;  // of the rows served so far
+  bool open = true, found = false;
+  uint32_t bits = 0;
+  for (int64_t base = 0; base < a.rows; base += kPlanBlock) {
+    const int64_t row = base + tid;
+    const bool in = row < a.rows;
+    const int64_t n_raw = in ? a.new_lens[row] : 0, c = in ? a.cached_lens[row] : 0;
+    const bool valid = n_raw >= 0 && c >= 0 && c + n_raw <= reach;
+    const int64_t n = valid ? n_raw : 0;
+    // (32-bit quotients: a valid row's lengths are below 2^31)
+    const uint32_t have = valid ? (static_cast<uint32_t>(c) + ps - 1) / ps : 0u;
+    const uint32_t need = valid ? (static_cast<uint32_t>(c + n) + ps - 1) / ps - have : 0u;
+    int64_t tok = wave_scan(n, lane), pag = wave_scan(static_cast<int64_t>(need), lane);
+    __syncthreads();  // the previous 256 rows' shared values are read
+    if (lane == kWave - 1) {
+      sums[0][wave] = tok;
+      sums[1][wave] = pag;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w)
+      if (w < wave) {
+        tok += sums[0][w];
+        pag += sums[1][w];
+      }
+    tok += tokens;
+    pag += pages;
+    const bool served = open && tok <= a.num_tokens && pag <= avail;
+    const int64_t top_t = wave_max64(served ? tok : 0), top_p = wave_max64(served ? pag : 0);
+    if (lane == 0) {
+      tops[0][wave] = top_t;
+      tops[1][wave] = top_p;
+    }
+    row_new[tid] = served ? static_cast<int>(n) : 0;
+    row_cached[tid] = static_cast<int>(c);
+    row_page[tid] = static_cast<int>(served ? pag - need : 0);
+    open = __syncthreads_and(served);
+    const int64_t before = tokens;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+      tokens = max(tokens, tops[0][w]);
+      pages = max(pages, tops[1][w]);
+    }
+    const int end = static_cast<int>(served ? tok : tokens);
+    ends[tid] = end;
+    if (writer && in) {
+      a.cu[row + 1] = end;
+      a.seq_lens[row] = static_cast<int32_t>(c + (served ? n : 0));
+      if (!valid) bits |= MAS_ERRBIT_POSITION;
+      else if (!served && n > 0) bits |= MAS_ERRBIT_POOL;
+    }
+    __syncthreads();
+    if (t >= before && t < tokens) {  // this thread's token lies in these rows
+      found = true;
+      int lo = 0, hi = kPlanBlock - 1;  // the first row whose end is past t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (ends[mid] > t) hi = mid;
+        else lo = mid + 1;
+      }
+      const int64_t r = base + lo;
+      const uint32_t cached = static_cast<uint32_t>(row_cached[lo]);
+      const uint32_t pos = cached + static_cast<uint32_t>(static_cast<int>(t) - (ends[lo] - row_new[lo]));
+      const uint32_t first = (cached + ps - 1) / ps, block = pos / ps, entry = pos - block * ps;
+      int32_t* const table = a.tables + r * a.bt_stride;
+      int32_t page;
+      if (block < first) {
+        page = table[block];
+      } else {
+        int64_t at = head_at + row_page[lo] + (block - first);
+        if (at >= a.ring) at -= a.ring;
+        page = a.free_pages[at];
+        if (entry == 0) table[block] = page;
+      }
+      a.positions[t] = static_cast<int32_t>(pos);
+      a.batch_indices[t] = static_cast<int32_t>(r);
+      a.slots[t] = page < 0 ? -1 : static_cast<int64_t>(page) * a.page_size + entry;
+      if (page < 0) report(a.err, MAS_ERRBIT_PAGE);
+    }
+    if (!writer && tokens >= last_t) break;  // uniform: this workgroup's tokens are written
+  }
+  if (!found && t < a.num_tokens) {  // a padding token
+    a.positions[t] = 0;
+    a.batch_indices[t] = -1;
+    a.slots[t] = -1;
+  }
+  if (writer) {
+    if (bits != 0) report(a.err, bits);
+    if (tid == 0) {
+      a.cu[0] = 0;
+      a.range_out[0] = head + pages;
+      a.range_out[1] = tail;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace mas
+
+extern "C" int mas_plan_step(int32_t* positions, int32_t* batch_indices, int64_t* slot_mapping, int32_t* cu_seqlens_q,
+                             int32_t* seq_lens, int64_t* free_range_out, int32_t* block_tables,
+                             int64_t block_table_stride, int64_t max_blocks, const int32_t* new_lens,
+                             const int32_t* cached_lens, int64_t rows, const int32_t* free_pages,
+                             int64_t num_free_pages, const int64_t* free_range, int64_t page_size, int64_t num_tokens,
+                             uint32_t* err, hipStream_t stream) {
+  using namespace mas;
+  if (rows < 0 || num_tokens < 0 || page_size <= 0 || max_blocks < 0 || num_free_pages < 0)
+    return MAS_ERR_INVALID_VALUE;
+  if (cu_seqlens_q == nullptr || free_range == nullptr || free_range_out == nullptr || free_range == free_range_out)
+    return MAS_ERR_INVALID_VALUE;
+  if (rows > 0 && (new_lens == nullptr || cached_lens == nullptr || seq_lens == nullptr || seq_lens == new_lens ||
+                   seq_lens == cached_lens || (max_blocks > 0 && block_tables == nullptr)))
+    return MAS_ERR_INVALID_VALUE;
+  if (num_tokens > 0 && (positions == nullptr || batch_indices == nullptr || slot_mapping == nullptr))
+    return MAS_ERR_INVALID_VALUE;
+  if (num_free_pages > 0 && free_pages == nullptr) return MAS_ERR_INVALID_VALUE;
+  // positions, token counts and pages are 32-bit numbers
+  if (page_size > (1 << 30) || max_blocks * page_size > (int64_t{1} << 30) || num_tokens > INT32_MAX - 1 ||
+      rows > INT32_MAX - 1 || num_free_pages > INT32_MAX)
+    return MAS_ERR_UNSUPPORTED;
+  const StepArgs a{positions, batch_indices, slot_mapping, cu_seqlens_q, seq_lens, free_range_out, block_tables,
+                   block_table_stride, max_blocks, new_lens, cached_lens, rows, free_pages, num_free_pages, free_range,
+                   page_size, num_tokens, err};
+  const int64_t blocks = num_tokens > 0 ? cdiv(num_tokens, kPlanBlock) : 1;
+  hipLaunchKernelGGL(plan_step, dim3(static_cast<uint32_t>(blocks)), dim3(kPlanBlock), 0, stream, a);
+  return launch_status();
+}

@@ -10,6 +10,8 @@ reference makes, not from any kernel source:
   the llama-4 query scale, the paged KV append (block-table and slot forms), the embedding gather
   and the step-input placeholder fill, paged decode and causal context attention, and the RoPE
   table builders.
+- ``fp4``: the 4-bit KV cache's quantize and its inverse, decode and context attention over it, and the step
+  plan, in 64 bits.
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and the ``cpu_baseline`` leg of ``bench.py`` may
 import this package, and only as the reference that results are compared against or as the timed
@@ -40,4 +42,4 @@ library is absent and the reference has no tests or fixtures, so agreement with 
 bit for bit is "parity unpinned"; the oracle fixes one documented rounding order per op and the
 GPU parity tests hold the kernels to it within the stated tolerances.
 """
-from . import numerics, ops  # noqa: F401
+from . import fp4, numerics, ops  # noqa: F401
