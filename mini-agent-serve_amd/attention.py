@@ -374,6 +374,12 @@ def batch_decode_with_fp4_kv_cache(query: torch.Tensor, kv_cache, workspace_buff
                                                  float(bmm1_scale), float(bmm2_scale), out, kv_layout, qs, qs_host,
                                                  error_flags)
         return out
+    if _lib.direct is not None and (st := _lib.direct.decode_attention_fp4(
+            query, kv_cache, workspace_buffer, block_tables, seq_lens, bmm1_scale, bmm2_scale, out, kv_layout,
+            error_flags, out_quant_scale)) is not None:
+        if st:
+            _lib.check(st, "batch_decode_with_fp4_kv_cache")
+        return out
     _decode_fp4(query, kv_cache, workspace_buffer, block_tables, seq_lens, bmm1_scale, bmm2_scale, out, kv_layout,
                 error_flags, out_quant_scale)
     return out
@@ -430,6 +436,12 @@ def batch_context_with_fp4_kv_cache(query: torch.Tensor, kv_cache, workspace_buf
         torch.ops.mas.paged_context_attention_fp4(query, *kv_cache, workspace_buffer, block_tables, seq_lens,
                                                   cum_seq_lens_q, int(max_q_len), int(max_kv_len), float(bmm1_scale),
                                                   float(bmm2_scale), out, kv_layout, qs, qs_host, error_flags)
+        return out
+    if _lib.direct is not None and (st := _lib.direct.context_attention_fp4(
+            query, kv_cache, workspace_buffer, block_tables, seq_lens, cum_seq_lens_q, max_q_len, max_kv_len,
+            bmm1_scale, bmm2_scale, out, kv_layout, error_flags, out_quant_scale)) is not None:
+        if st:
+            _lib.check(st, "batch_context_with_fp4_kv_cache")
         return out
     _context_fp4(query, kv_cache, workspace_buffer, block_tables, seq_lens, cum_seq_lens_q, max_q_len, max_kv_len,
                  bmm1_scale, bmm2_scale, out, kv_layout, error_flags, out_quant_scale)

@@ -284,6 +284,11 @@ def append_paged_kv_cache_fp4(append_key: torch.Tensor, append_value: torch.Tens
         torch.ops.mas.append_paged_kv_cache_fp4(append_key, append_value, batch_indices, positions, *kv_cache,
                                                 kv_indices, kv_indptr, kv_layout, error_flags)
         return
+    if _lib.direct is not None and (st := _lib.direct.append_fp4(append_key, append_value, batch_indices, positions, kv_cache,
+                                                                 kv_indices, kv_indptr, kv_layout, error_flags)) is not None:
+        if st:
+            _lib.check(st, "append_paged_kv_cache_fp4")
+        return
     _append_fp4(append_key, append_value, batch_indices, positions, kv_cache, kv_indices, kv_indptr, kv_layout,
                 error_flags)
 
@@ -313,6 +318,11 @@ def store_kv_slots_fp4(key: torch.Tensor, value: torch.Tensor, kv_cache, slot_ma
     if torch.compiler.is_compiling():
         torch.ops.mas.store_kv_slots_fp4(key, value, *kv_cache, slot_mapping, kv_layout, error_flags)
         return
+    if _lib.direct is not None and (st := _lib.direct.store_slots_fp4(key, value, kv_cache, slot_mapping, kv_layout,
+                                                                      error_flags)) is not None:
+        if st:
+            _lib.check(st, "store_kv_slots_fp4")
+        return
     _slots_fp4("store", key, value, kv_cache, slot_mapping, kv_layout, error_flags)
 
 
@@ -328,6 +338,11 @@ def load_kv_slots_fp4(kv_cache, slot_mapping: torch.Tensor, kv_layout: str = "NH
         value = torch.empty(shape, dtype=torch.bfloat16, device=slot_mapping.device) if value is None else value
     if torch.compiler.is_compiling():
         torch.ops.mas.load_kv_slots_fp4(key, value, *kv_cache, slot_mapping, kv_layout, error_flags)
+        return key, value
+    if _lib.direct is not None and (st := _lib.direct.load_slots_fp4(key, value, kv_cache, slot_mapping, kv_layout,
+                                                                     error_flags)) is not None:
+        if st:
+            _lib.check(st, "load_kv_slots_fp4")
         return key, value
     _slots_fp4("load", key, value, kv_cache, slot_mapping, kv_layout, error_flags)
     return key, value

@@ -118,5 +118,10 @@ def plan_step(new_lens: torch.Tensor, cached_lens: torch.Tensor, block_tables: t
         torch.ops.mas.plan_step(new_lens, cached_lens, block_tables, free_pages, free_range, int(page_size), *out,
                                 error_flags)
         return StepTables(*out)
+    if _lib.direct is not None and (st := _lib.direct.plan_step(new_lens, cached_lens, block_tables, free_pages,
+                                                                free_range, page_size, out, error_flags)) is not None:
+        if st:
+            _lib.check(st, "plan_step")
+        return out if type(out) is StepTables else StepTables(*out)
     _plan(new_lens, cached_lens, block_tables, free_pages, free_range, page_size, out, error_flags)
     return StepTables(*out)

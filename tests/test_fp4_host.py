@@ -200,3 +200,22 @@ def test_ops_are_registered(mas):
     names = {n for n in dir(torch.ops.mas) if not n.startswith("_")}
     assert {"append_paged_kv_cache_fp4", "store_kv_slots_fp4", "load_kv_slots_fp4", "paged_decode_attention_fp4",
             "paged_context_attention_fp4", "plan_step"} <= names
+
+
+def test_direct_calls_leave_other_forms_to_the_wrappers(mas):
+    """On the CPU no form is taken, whatever the arguments are, and a refusal costs little."""
+    import timeit
+    mas.load_library()
+    d = mas._lib.direct
+    if d is None:
+        pytest.skip("direct_calls.so not built")
+    c = mas.page.fp4_kv_cache(3, 16, 2, 64, "cpu")
+    x, i = torch.zeros(1, 2, 64, dtype=BF16), torch.zeros(1, dtype=I64)
+    calls = [lambda: d.store_slots_fp4(x, x, c, i, "HND", None), lambda: d.load_slots_fp4(x, x, c, i, "HND", None),
+             lambda: d.append_fp4(*[None] * 9), lambda: d.decode_attention_fp4(*[None] * 11),
+             lambda: d.context_attention_fp4(*[None] * 14), lambda: d.plan_step(*[None] * 8),
+             lambda: d.plan_step(i.int(), i.int(), i.int().view(1, 1), i.int(), i, 16, mas.step.step_tables(1, 1, "cpu"), None),
+             lambda: d.plan_step(), lambda: d.append_fp4(x, x, i, i, c[:2], i, i, "HND", None)]
+    for call in calls:
+        assert call() is None
+        assert min(timeit.repeat(call, number=200, repeat=10)) / 200 < 2e-5
