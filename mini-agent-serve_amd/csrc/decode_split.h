@@ -114,7 +114,8 @@ __device__ __forceinline__ float wave_max(float v) {
 
 // One wavefront per (query head, row): lane s reads split s's (max, sum) (64 splits per pass), the
 // weights are broadcast with readlane, and each lane accumulates D / 64 head-dim elements.
-template <int D>
+// kSplitLen: the split length of a row, as the split kernel takes it.
+template <int D, int (*kSplitLen)(const DecodeArgs&, int) = row_split_len>
 __global__ __launch_bounds__(64) void decode_attn_combine(DecodeArgs a) {
   constexpr int DPL = D / 64;  // head-dim elements per lane
   const int lane = threadIdx.x;
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(64) void decode_attn_combine(DecodeArgs a) {
   // reported at the end: a global atomic here would turn the loads below into waits on every load
   const bool len_bad = raw < 0 || raw > cap;
   const int L = static_cast<int>(raw < 0 ? 0 : (raw > cap ? cap : raw));
-  const int split_len = row_split_len(a, L);
+  const int split_len = kSplitLen(a, L);
   const int nsplit = (L + split_len - 1) / split_len;
   if (nsplit == 1) {  // the split kernel wrote this row's output
     if (len_bad && h == 0 && lane == 0) report(a.err, MAS_ERRBIT_POSITION);

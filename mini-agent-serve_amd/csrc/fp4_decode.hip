@@ -6,8 +6,9 @@
 // k_p and v_p the values the codes stand for; fp32 sums, rounded once to bf16 (decode attention over the
 // bf16 cache, devstral2.py:184-196, on another cache format).
 //
-// Split-KV as there (decode_split.h): a wavefront per (kv head, split, row), then the merge of the splits.
-// A split is walked in steps of 32 positions, two 16-position tiles, entirely in registers:
+// Split-KV as there (decode_split.h): a workgroup of four wavefronts per (kv head, split, row), then the merge of
+// the splits. The wavefronts take the split's steps of 32 positions (two 16-position tiles) in turn, each entirely
+// in registers, and add up through LDS at the end:
 //   S^T = K Q^T on v_mfma_f32_16x16x32_bf16: lane (n, r) loads quarter r of key row n (32 codes of head_dim 128, one
 //     block) and decodes it (v_cvt_scalef32_pk_bf16_fp4, exact); the columns of B are the kv head's query heads, with
 //     the head dim numbered as the lanes hold it. (The scaled MFMAs take e2m1 operands as they lie in memory, but
@@ -29,6 +30,28 @@ namespace {
 
 constexpr float kSumMost = 256.f;
 
+// `bytes` of memory at a wavefront-uniform address as a raw buffer resource (dword 3 = the 32-bit data format that
+// untyped buffer loads take on gfx9): loads take a scalar base, a 32-bit lane offset and a scalar one, with no vector
+// arithmetic, and give zeros past the end.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, bytes, 0x00020000);
+}
+
+constexpr int kWaves = 4;
+constexpr int kStep = 32;                    // positions a wavefront takes at a time
+constexpr int kRound = kWaves * kStep;       // and a workgroup
+constexpr int kMaxSplitLen = 512;            // positions per split, at most, while max_splits reach
+constexpr int kMaxSplits = 128;
+
+// A row's split length: its share of row_target splits, in whole rounds, at most kMaxSplitLen; and such that its splits
+// fit the grid and the workspace.
+__device__ __forceinline__ int fp4_split_len(const DecodeArgs& a, int L) {
+  const int rounds = (L + kRound - 1) / kRound;
+  const int share = (rounds + a.row_target - 1) / a.row_target;
+  const int least = (rounds + a.max_splits - 1) / a.max_splits;
+  return kRound * max(max(min(share, kMaxSplitLen / kRound), least), 1);
+}
+
 struct Fp4DecodeArgs : DecodeArgs {
   Fp4Cache c;
 };
@@ -46,33 +69,39 @@ struct Fp4Loads {
   int count[2];  // valid positions of each tile (wavefront-uniform)
 };
 
-template <int D, int kHeads>
-__global__ __launch_bounds__(64 * kHeads, D <= 128 ? 3 : 1) void fp4_decode_split(Fp4DecodeArgs a) {
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_split(Fp4DecodeArgs a) {
   using Loads = Fp4Loads<D>;
   constexpr int EL = D / 16;     // head-dim elements per lane of the value operand: EL n ..
   constexpr int NB = EL / 2;     // their code bytes per position
-  constexpr int kStep = 32;
   const int lane = threadIdx.x & 63;
   const int wave = wave_id_uniform();
-  const int kvh = blockIdx.x * kHeads + wave;
+  const int kvh = blockIdx.x;
   const int b = blockIdx.z;
   // the splits of row b rotated over the grid, as in the bf16 kernel: rows shorter than the table have only
   // their first splits to do, which would all land on the same XCDs
   const unsigned turn = gridDim.y & 1 ? 0u : blockIdx.z + (blockIdx.z >> 2);
   const int split = static_cast<int>((blockIdx.y + turn) % gridDim.y);
   const int L = kv_len(a, b);
-  const int split_len = row_split_len(a, L);
+  const int split_len = fp4_split_len(a, L);
   const int start = split * split_len;
   if (start >= L) return;
   const int end = min(start + split_len, L);
   const int G = a.group;
   const int n = lane & 15, r = lane >> 4;
 
-  // Block-table entries of the split: lane i holds entry first + i.
-  const int32_t* bt = a.block_tables + b * a.bt_stride;
-  int first = start >> a.log2_page;
-  auto load_entries = [&] { return bt[min(static_cast<int64_t>(first + lane), a.max_blocks - 1)]; };
-  int entries = load_entries();
+  // A tile's page id is a scalar load, a step ahead of the tile's own loads (constant address space, so that it
+  // counts on another counter than those: a vector load here would wait for all of them).
+  const auto bt = (const __attribute__((address_space(4))) int32_t*)(a.block_tables + b * a.bt_stride);
+  const int last_entry = (end - 1) >> a.log2_page;
+  struct Ids {
+    int32_t page[2];
+  };
+  auto fetch = [&](int pos) {
+    return Ids{{bt[min(pos >> a.log2_page, last_entry)], bt[min((pos + 16) >> a.log2_page, last_entry)]}};
+  };
+  const int begin = start + wave * kStep;  // this wavefront's first step
+  Ids ids = fetch(begin);
   // B operands of S^T = K Q^T: head n, head-dim elements D / 4 r + 8 j + 0..7 (zeros past the group)
   constexpr int KJ = D / 32;
   bf16x8 q[KJ];
@@ -98,62 +127,62 @@ __global__ __launch_bounds__(64 * kHeads, D <= 128 ? 3 : 1) void fp4_decode_spli
   const uint8_t* const ks_head = a.c.k_scale + kvh * a.c.scale_head_stride;
   const uint8_t* const vs_head = a.c.v_scale + kvh * a.c.scale_head_stride;
 
+  const uint32_t pages_u32 = static_cast<uint32_t>(min(a.c.num_pages, static_cast<int64_t>(INT32_MAX)));
   bool bad = false;
+  // Issues the loads of the step at `pos`, whose pages are in `ids`, and fetches the next step's.
   auto issue = [&](Loads& st, int pos) {
-    int64_t at[2], sat[2];  // byte offsets of the tiles' first rows and powers
+    // the tiles' rows, as many as are valid (the others arrive as zeros), and their head's powers
+    __amdgpu_buffer_rsrc_t k_at[2], v_at[2], ks_at[2], vs_at[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int p = pos + 16 * t;
-      const int pc = p < end ? p : end - 1;  // a tile past the end reads the last position's page
-      const int entry = pc >> a.log2_page;
-      if (entry - first >= 64) {  // uniform
-        first = entry;
-        entries = load_entries();
-      }
-      const int32_t page = __builtin_amdgcn_readlane(entries, entry - first);
-      const bool ok = page >= 0 && page < a.c.num_pages;
-      st.count[t] = ok ? max(0, min(16, end - p)) : 0;
+      const uint32_t page = static_cast<uint32_t>(ids.page[t]);
+      const bool ok = page < pages_u32;
+      const int count = __builtin_amdgcn_readfirstlane(ok ? max(0, min(16, end - p)) : 0);
+      st.count[t] = count;
       bad |= !ok;
-      const int64_t pg = ok ? page : 0;
-      const uint32_t slot = static_cast<uint32_t>(pc & mask & ~15);
-      at[t] = pg * a.c.page_stride + static_cast<int64_t>(slot) * es;
-      sat[t] = pg * a.c.scale_page_stride + slot;
+      const uint32_t slot = static_cast<uint32_t>(p & mask);
+      const int64_t at = static_cast<int64_t>(ok ? page : 0u) * a.c.page_stride + static_cast<int64_t>(slot * es);
+      const int64_t sat = static_cast<int64_t>(ok ? page : 0u) * a.c.scale_page_stride + slot;
+      const int bytes = count * static_cast<int>(es), sbytes = count > 0 ? static_cast<int>(D / kFp4Block * ps - slot) : 0;
+      k_at[t] = buffer_of(k_head + at, bytes);
+      v_at[t] = buffer_of(v_head + at, bytes);
+      ks_at[t] = buffer_of(ks_head + sat, sbytes);
+      vs_at[t] = buffer_of(vs_head + sat, sbytes);
     }
+    ids = fetch(pos + kRound);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t* src = k_head + at[t] + k_off;
       if constexpr (D == 64) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(k_at[t], k_off, 0, 0);
         st.k[t][0] = x[0];
         st.k[t][1] = x[1];
       } else {
 #pragma unroll
         for (int h = 0; h < D / 128; ++h) {
-          const u32x4 x = load_cached(src + 16 * h);
+          const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(k_at[t], k_off + 16 * h, 0, 0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) st.k[t][4 * h + i] = x[i];
         }
       }
 #pragma unroll
-      for (int h = 0; h < Loads::KP; ++h) st.ks[t][h] = (ks_head + sat[t])[ks_off + h * ps];
+      for (int h = 0; h < Loads::KP; ++h) st.ks[t][h] = __builtin_amdgcn_raw_buffer_load_b8(ks_at[t], ks_off, h * ps, 0);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t* base = v_head + at[t];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* src = base + static_cast<int64_t>(i) * es + v_off;
         if constexpr (D == 64) {
-          st.v[t][i][0] = *reinterpret_cast<const uint16_t*>(src);
+          st.v[t][i][0] = __builtin_amdgcn_raw_buffer_load_b16(v_at[t], v_off, i * es, 0);
         } else if constexpr (D == 128) {
-          st.v[t][i][0] = *reinterpret_cast<const uint32_t*>(src);
+          st.v[t][i][0] = __builtin_amdgcn_raw_buffer_load_b32(v_at[t], v_off, i * es, 0);
         } else {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+          const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(v_at[t], v_off, i * es, 0);
           st.v[t][i][0] = x[0];
           st.v[t][i][1] = x[1];
         }
       }
-      st.vs[t] = *reinterpret_cast<const uint32_t*>(vs_head + sat[t] + vs_off);
+      st.vs[t] = __builtin_amdgcn_raw_buffer_load_b32(vs_at[t], vs_off, 0, 0);
     }
   };
 
@@ -178,11 +207,8 @@ __global__ __launch_bounds__(64 * kHeads, D <= 128 ? 3 : 1) void fp4_decode_spli
         const int left = st.count[t] - 4 * r;  // valid positions of this lane's four
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (j >= left) {
-            s[t][j] = kNegInf;
-#pragma unroll
-            for (int x = 0; x < Loads::VW; ++x) st.v[t][j][x] = 0u;
-          }
+          if (j >= left) s[t][j] = kNegInf;
+        // (the values' codes are zeros there, but a power of 255 would make them NaN)
         st.vs[t] = left >= 4 ? st.vs[t] : left <= 0 ? 0u : st.vs[t] & ((1u << (8 * left)) - 1u);
       }
     }
@@ -263,56 +289,78 @@ __global__ __launch_bounds__(64 * kHeads, D <= 128 ? 3 : 1) void fp4_decode_spli
   };
 
   // Two load buffers used in turn: a step is computed while the next one's loads are in flight.
-  const int nsteps = (end - start + kStep - 1) / kStep;
-  Loads ld0, ld1;
-  issue(ld0, start);
-  int i = 0;
-  for (; i + 2 < nsteps; i += 2) {
-    issue(ld1, start + (i + 1) * kStep);
-    compute(ld0);
-    issue(ld0, start + (i + 2) * kStep);
-    compute(ld1);
-  }
-  if (i + 1 < nsteps) {
-    issue(ld1, start + (i + 1) * kStep);
-    compute(ld0);
-    compute(ld1);
-  } else {
-    compute(ld0);
+  const int nsteps = begin < end ? (end - begin + kRound - 1) / kRound : 0;
+  if (nsteps > 0) {
+    Loads ld0, ld1;
+    issue(ld0, begin);
+    int i = 0;
+    for (; i + 2 < nsteps; i += 2) {
+      issue(ld1, begin + (i + 1) * kRound);
+      compute(ld0);
+      issue(ld0, begin + (i + 2) * kRound);
+      compute(ld1);
+    }
+    if (i + 1 < nsteps) {
+      issue(ld1, begin + (i + 1) * kRound);
+      compute(ld0);
+      compute(ld1);
+    } else {
+      compute(ld0);
+    }
   }
   if (__builtin_amdgcn_ballot_w64(bad) != 0 && lane == 0) report(a.err, MAS_ERRBIT_PAGE);
 
+  // ---- the wavefronts' sums: each brings its own to the workgroup's reference and puts them into LDS
+  constexpr int OROW = D + 4;  // floats per LDS row: the 16 heads' rows start 4 banks apart
+  __shared__ __align__(16) float o_lds[kWaves][16 * OROW];
+  __shared__ float m_lds[kWaves][16], l_lds[kWaves][16], m_all_lds[16];
   l_run += __shfl_xor(l_run, 16);
   l_run += __shfl_xor(l_run, 32);
-  if (n >= G) return;
-  const int h = kvh * G + n;
-  if (L <= split_len) {  // the row's only split: its output
-    const float sc = l_run > 0.f ? a.out_scale / l_run : 0.f;
+  if (r == 0) m_lds[wave][n] = m_run;
+  __syncthreads();
+  const float m_all = fmaxf(fmaxf(m_lds[0][n], m_lds[1][n]), fmaxf(m_lds[2][n], m_lds[3][n]));
+  // (a wavefront without a finite score has sums of zero, or NaN ones where its scores are)
+  const float factor = m_run == kNegInf ? (l_run != l_run ? l_run : 0.f) : __builtin_amdgcn_exp2f(m_run - m_all);
+  if (n < G) {
+    if (r == 0) l_lds[wave][n] = l_run * factor;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < EL; e += 4) {
-        const float y[4] = {acc[e][j] * sc, acc[e + 1][j] * sc, acc[e + 2][j] * sc, acc[e + 3][j] * sc};
-        store_output<4>(a, b, h, EL * (4 * r + j) + e, y);
-      }
-    return;
+      for (int e = 0; e < EL; e += 4)
+        *reinterpret_cast<f32x4*>(&o_lds[wave][n * OROW + EL * (4 * r + j) + e]) =
+            f32x4{acc[e][j] * factor, acc[e + 1][j] * factor, acc[e + 2][j] * factor, acc[e + 3][j] * factor};
   }
-  const int64_t at = (static_cast<int64_t>(b) * a.hq + h) * a.max_splits + split;
+  if (wave == 0 && r == 0) m_all_lds[n] = m_all;
+  __syncthreads();
+  constexpr int kVecs = D / 4;  // 16-byte pieces per head row
+  for (int i = threadIdx.x; i < G * kVecs; i += 64 * kWaves) {
+    const int g = i / kVecs, c = i % kVecs;
+    f32x4 o = *reinterpret_cast<const f32x4*>(&o_lds[0][g * OROW + 4 * c]);
+    float l = l_lds[0][g];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int e = 0; e < EL; e += 4)
-      __builtin_nontemporal_store(f32x4{acc[e][j], acc[e + 1][j], acc[e + 2][j], acc[e + 3][j]},
-                                  reinterpret_cast<f32x4*>(a.part_o + at * D + EL * (4 * r + j) + e));
-  if (r == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m_run, l_run};
+    for (int w = 1; w < kWaves; ++w) {
+      o += *reinterpret_cast<const f32x4*>(&o_lds[w][g * OROW + 4 * c]);
+      l += l_lds[w][g];
+    }
+    const int h = kvh * G + g;
+    if (L <= split_len) {  // the row's only split: its output
+      const float sc = l > 0.f ? a.out_scale / l : 0.f;
+      const float y[4] = {o[0] * sc, o[1] * sc, o[2] * sc, o[3] * sc};
+      store_output<4>(a, b, h, 4 * c, y);
+    } else {
+      const int64_t at = (static_cast<int64_t>(b) * a.hq + h) * a.max_splits + split;
+      __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(a.part_o + at * D + 4 * c));
+      if (c == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m_all_lds[g], l};
+    }
+  }
 }
 
 template <int D>
 int launch_fp4_decode(const Fp4DecodeArgs& a, int64_t batch, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(a.hk), static_cast<uint32_t>(a.max_splits), static_cast<uint32_t>(batch));
-  hipLaunchKernelGGL((fp4_decode_split<D, 1>), grid, dim3(64), 0, s, a);
+  hipLaunchKernelGGL(fp4_decode_split<D>, grid, dim3(64 * kWaves), 0, s, a);
   if (const int st = launch_status(); st != MAS_OK) return st;
-  hipLaunchKernelGGL((decode_attn_combine<D>), dim3(static_cast<uint32_t>(a.hq), static_cast<uint32_t>(batch)),
+  hipLaunchKernelGGL((decode_attn_combine<D, fp4_split_len>), dim3(static_cast<uint32_t>(a.hq), static_cast<uint32_t>(batch)),
                      dim3(64), 0, s, a);
   return launch_status();
 }
@@ -363,10 +411,16 @@ extern "C" int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int
   if (!aligned16(q) || !aligned16(out) || q_stride % 8 != 0 || q_head_stride % 8 != 0 || out_stride % 8 != 0 ||
       out_head_stride % 8 != 0 || !aligned16(workspace))
     return MAS_ERR_MISALIGNED;
-  DecodeSplits sp{};
-  if (const int st = decode_splits(batch, num_q_heads, num_kv_heads, head_dim, cap, workspace, workspace_bytes, &sp);
-      st != MAS_OK)
-    return st == kWorkspaceTooSmall ? MAS_ERR_INVALID_VALUE : st;
+  // Splits wanted per row: four workgroups per CU over the (row, kv head) pairs. The longest row a table can hold
+  // then has the more of those and of kMaxSplitLen-position splits; fewer where the workspace holds fewer partials.
+  int cus = 0;
+  if (workspace == nullptr) return MAS_ERR_INVALID_VALUE;
+  if (const int st = device_cu_count(&cus); st != MAS_OK) return st;
+  const int64_t target = std::max<int64_t>(1, 4 * static_cast<int64_t>(cus) / (batch * num_kv_heads));
+  const int64_t held = workspace_bytes / decode_workspace_bytes(batch, num_q_heads, head_dim, 1);
+  if (held < 1) return MAS_ERR_INVALID_VALUE;
+  const int64_t splits = std::max<int64_t>(
+      1, std::min({std::max(std::min(target, cdiv(cap, kRound)), cdiv(cap, kMaxSplitLen)), int64_t{kMaxSplits}, held}));
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_stride;
   a.q_head_stride = q_head_stride;
@@ -379,13 +433,12 @@ extern "C" int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int
   a.hk = static_cast<int>(num_kv_heads);
   a.group = static_cast<int>(group);
   while ((int64_t{1} << a.log2_page) < page_size) ++a.log2_page;
-  a.split_len = static_cast<int>(sp.split_len);
-  a.row_target = sp.row_target;
-  a.max_splits = static_cast<int>(sp.splits);
+  a.row_target = static_cast<int>(target);
+  a.max_splits = static_cast<int>(splits);
   a.scale_log2 = bmm1_scale * 1.4426950408889634f;
   a.out_scale = bmm2_scale;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + batch * num_q_heads * sp.splits * head_dim;
+  a.part_ml = a.part_o + batch * num_q_heads * splits * head_dim;
   a.out = out;
   a.out_stride = out_stride;
   a.out_head_stride = out_head_stride;
