@@ -40,7 +40,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* p, in
 constexpr int kWaves = 4;
 constexpr int kStep = 32;                    // positions a wavefront takes at a time
 constexpr int kRound = kWaves * kStep;       // and a workgroup
-constexpr int kMaxSplitLen = 512;            // positions per split, at most, while max_splits reach
+constexpr int kMaxSplitLen = 1024;           // positions per split, at most, while max_splits reach
 constexpr int kMaxSplits = 128;
 
 // A row's split length: its share of row_target splits, in whole rounds, at most kMaxSplitLen; and such that its splits
@@ -53,6 +53,8 @@ __device__ __forceinline__ int fp4_split_len(const DecodeArgs& a, int L) {
 }
 
 struct Fp4DecodeArgs : DecodeArgs {
+  int batch;
+  int heads_share;  // kv heads' codes share 128-byte lines
   Fp4Cache c;
 };
 
@@ -76,16 +78,32 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_spli
   constexpr int NB = EL / 2;     // their code bytes per position
   const int lane = threadIdx.x & 63;
   const int wave = wave_id_uniform();
-  const int kvh = blockIdx.x;
-  const int b = blockIdx.z;
-  // the splits of row b rotated over the grid, as in the bf16 kernel: rows shorter than the table have only
-  // their first splits to do, which would all land on the same XCDs
-  const unsigned turn = gridDim.y & 1 ? 0u : blockIdx.z + (blockIdx.z >> 2);
-  const int split = static_cast<int>((blockIdx.y + turn) % gridDim.y);
+  // Workgroups go to the XCDs round-robin by id. Where heads share 128-byte lines (the NHD layout up to head_dim 128),
+  // all kv heads of a (split, row) item run on one XCD, so that a line comes from memory once: 64 rows of up to 8192
+  // positions 102 -> 67 us. Elsewhere the heads are dealt out, which balances the XCDs better (HND 62 -> 60 us). A row
+  // shorter than the table has only its first splits to do: those of row b are rotated by b + b / 4 over the items.
+  const unsigned id = blockIdx.x, hk = a.hk, queue = id / kXcds;
+  const unsigned item = a.heads_share ? queue / hk * kXcds + id % kXcds : id / hk;
+  const int kvh = static_cast<int>(a.heads_share ? queue % hk : id % hk);
+  const unsigned b_of = item / a.max_splits, y = item - b_of * a.max_splits;
+  const int b = static_cast<int>(b_of);
+  if (b >= a.batch) return;
+  const int split = static_cast<int>((y + (a.max_splits & 1 ? 0u : b_of + (b_of >> 2))) % a.max_splits);
   const int L = kv_len(a, b);
   const int split_len = fp4_split_len(a, L);
   const int start = split * split_len;
-  if (start >= L) return;
+  if (split == 0 && kvh == 0 && threadIdx.x == 0) {
+    const int64_t raw = a.seq_lens[b];
+    if (raw < 0 || raw > a.max_blocks << a.log2_page) report(a.err, MAS_ERRBIT_POSITION);
+  }
+  if (start >= L) {
+    if (split == 0) {  // a row with no position
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = threadIdx.x; i < a.group * (D / 4); i += 64 * kWaves)
+        store_output<4>(a, b, kvh * a.group + i / (D / 4), 4 * (i % (D / 4)), zero);
+    }
+    return;
+  }
   const int end = min(start + split_len, L);
   const int G = a.group;
   const int n = lane & 15, r = lane >> 4;
@@ -357,9 +375,11 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_spli
 
 template <int D>
 int launch_fp4_decode(const Fp4DecodeArgs& a, int64_t batch, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>(a.hk), static_cast<uint32_t>(a.max_splits), static_cast<uint32_t>(batch));
+  const int64_t items = cdiv(batch * a.max_splits, kXcds) * kXcds;  // (row, split), with the XCDs' remainder
+  if (items * a.hk > INT32_MAX) return MAS_ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<uint32_t>(items * a.hk));
   hipLaunchKernelGGL(fp4_decode_split<D>, grid, dim3(64 * kWaves), 0, s, a);
-  if (const int st = launch_status(); st != MAS_OK) return st;
+  if (const int st = launch_status(); st != MAS_OK || a.max_splits == 1) return st;  // (no row of several splits)
   hipLaunchKernelGGL((decode_attn_combine<D, fp4_split_len>), dim3(static_cast<uint32_t>(a.hq), static_cast<uint32_t>(batch)),
                      dim3(64), 0, s, a);
   return launch_status();
@@ -433,6 +453,8 @@ extern "C" int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int
   a.hk = static_cast<int>(num_kv_heads);
   a.group = static_cast<int>(group);
   while ((int64_t{1} << a.log2_page) < page_size) ++a.log2_page;
+  a.batch = static_cast<int>(batch);
+  a.heads_share = num_kv_heads > 1 && head_stride > -128 && head_stride < 128;
   a.row_target = static_cast<int>(target);
   a.max_splits = static_cast<int>(splits);
   a.scale_log2 = bmm1_scale * 1.4426950408889634f;

@@ -13,7 +13,7 @@
 // each lane moves 16-byte vectors, all loads issued before the stores.
 // Duplicate destinations (padding rows aimed at the model runner's sink block) are plain racing
 // stores of whole rows: one writer wins.
-#include "kv_dest.h"
+#include "device.h"
 
 namespace mas {
 namespace {
@@ -48,6 +48,47 @@ struct KvArgs {
   int vec_per_row;   // num_heads * head_dim / 8
   uint32_t* err;
 };
+
+// Resolves token t's (page, entry). Returns false when the token is skipped.
+template <bool kSlotForm>
+__device__ __forceinline__ bool resolve(const KvArgs& a, int64_t t, int64_t* page, int64_t* entry) {
+  if constexpr (kSlotForm) {
+    const int64_t slot = a.slots[t];
+    if (slot < 0) return false;
+    const int64_t pg = slot / a.page_size;
+    if (pg >= a.num_pages) {
+      report(a.err, MAS_ERRBIT_SLOT);
+      return false;
+    }
+    *page = pg;
+    *entry = slot - pg * a.page_size;
+    return true;
+  } else {
+    // Both per-token indices are loaded before either is checked, so the two loads overlap.
+    const int64_t b = a.batch_indices[t];
+    const int64_t p = a.positions[t];
+    const bool b_ok = b >= 0 && b < a.batch;
+    if (!b_ok || p < 0) {
+      report(a.err, b_ok ? MAS_ERRBIT_POSITION : MAS_ERRBIT_BATCH);
+      return false;
+    }
+    const int64_t first = a.kv_indptr[b];
+    const int64_t end = a.kv_indptr[b + 1];
+    const int64_t idx = first + p / a.page_size;
+    if (idx < 0 || idx >= a.num_indices || idx >= end) {
+      report(a.err, MAS_ERRBIT_PAGE);
+      return false;
+    }
+    const int64_t pg = a.kv_indices[idx];
+    if (pg < 0 || pg >= a.num_pages) {
+      report(a.err, MAS_ERRBIT_PAGE);
+      return false;
+    }
+    *page = pg;
+    *entry = p % a.page_size;
+    return true;
+  }
+}
 
 // Element offset of 16-byte vector v of a token's row, for a row made of heads of vec_per_head
 // vectors placed head_stride elements apart.

@@ -154,3 +154,37 @@ def test_views_of_a_larger_allocation(mas, dev):
     assert np.array_equal(wide[:, :heads * dim].reshape(n, heads, dim).float().cpu().numpy(),
                           fp4.dequantize(*fp4.quantize(bits(key))).astype(np.float32))
     assert bool((wide[:, heads * dim:] == 7.0).all())
+
+
+@pytest.mark.parametrize("heads,dim,ps,layout", [(2, 128, 16, "HND"), (9, 64, 32, "NHD"), (1, 64, 256, "HND")])
+def test_prompts(mas, dev, heads, dim, ps, layout):
+    """Prompts long enough for four tokens per wavefront: rows that start and end inside a group of four, at odd entries,
+    whose pages are not in order; some destinations outside the cache. Then the same rows by their slots, and back."""
+    new, cached = [1030, 1, 701, 2050, 3], [5, 17, 0, 31, ps - 1]
+    n, width = sum(new), max(-(-(c + m) // ps) for c, m in zip(cached, new))
+    pages = len(new) * width
+    tables = torch.randperm(pages, generator=torch.Generator().manual_seed(12)).to(torch.int32).reshape(len(new), width)
+    tables[2, 3] = -1
+    batch = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new)).to(torch.int32)
+    pos = torch.cat([torch.arange(c, c + m) for c, m in zip(cached, new)]).to(torch.int32)
+    batch[40] = -1
+    slots = [int(tables[b, p // ps]) * ps + p % ps if b >= 0 and int(tables[b, p // ps]) >= 0 else -1
+             for b, p in zip(batch.tolist(), pos.tolist())]
+    key, value = random_rows(13, n, heads, dim), random_rows(14, n, heads, dim)
+    cache, flags = _empty(mas, dev, pages, ps, heads, dim, layout), torch.zeros(1, dtype=torch.int32, device=dev)
+    indptr = (torch.arange(len(new) + 1) * width).to(torch.int32)
+    mas.append_paged_kv_cache_fp4(key.to(dev), value.to(dev), batch.to(dev), pos.to(dev), cache, tables.flatten().to(dev),
+                                  indptr.to(dev), None, layout, error_flags=flags)
+    want = _expect(cache, layout, slots, [bits(key), bits(value)], ps)
+    _same(cache, want)
+    lost = any(int(tables[b, p // ps]) < 0 for b, p in zip(batch.tolist(), pos.tolist()) if b >= 0)   # a row that long
+    assert int(flags) == (4 | 8 if lost else 4)
+    again, s = _empty(mas, dev, pages, ps, heads, dim, layout), torch.tensor(slots, device=dev)
+    flags.zero_()
+    mas.store_kv_slots_fp4(key.to(dev), value.to(dev), again, s, layout, error_flags=flags)
+    _same(again, want)
+    for x, y in zip((key, value), mas.load_kv_slots_fp4(again, s, layout, error_flags=flags)):
+        back = fp4.dequantize(*fp4.quantize(bits(x)))
+        back[torch.tensor(slots) < 0] = 0.0
+        assert np.array_equal(y.float().cpu().numpy().astype(np.float64), back)
+    assert int(flags) == 0
