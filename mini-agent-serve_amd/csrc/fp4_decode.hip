@@ -55,6 +55,7 @@ __device__ __forceinline__ int fp4_split_len(const DecodeArgs& a, int L) {
 struct Fp4DecodeArgs : DecodeArgs {
   int batch;
   int heads_share;  // kv heads' codes share 128-byte lines
+  int code_bytes, power_bytes;  // from a head's first code (power) to the end of its last page's, in a cache below 2 GiB
   Fp4Cache c;
 };
 
@@ -71,7 +72,10 @@ struct Fp4Loads {
   int count[2];  // valid positions of each tile (wavefront-uniform)
 };
 
-template <int D>
+// kWide: a cache tensor of 2 GiB or more, whose tiles each get buffer resources of their own; else one resource per tensor
+// serves every tile at a 32-bit scalar offset, which leaves the scalar unit a third of the work (it serves all of a CU's
+// wavefronts).
+template <int D, bool kWide>
 __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_split(Fp4DecodeArgs a) {
   using Loads = Fp4Loads<D>;
   constexpr int EL = D / 16;     // head-dim elements per lane of the value operand: EL n ..
@@ -147,60 +151,71 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_spli
 
   const uint32_t pages_u32 = static_cast<uint32_t>(min(a.c.num_pages, static_cast<int64_t>(INT32_MAX)));
   bool bad = false;
-  // Issues the loads of the step at `pos`, whose pages are in `ids`, and fetches the next step's.
+  // Issues the loads of the step at `pos`, whose pages are in `ids`, and fetches the next step's. Rows past the row's
+  // end, and all of a tile on a page id outside the cache (page 0 is read), are loaded and do not count.
+  const __amdgpu_buffer_rsrc_t k_all = buffer_of(k_head, a.code_bytes), v_all = buffer_of(v_head, a.code_bytes);
+  const __amdgpu_buffer_rsrc_t ks_all = buffer_of(ks_head, a.power_bytes), vs_all = buffer_of(vs_head, a.power_bytes);
   auto issue = [&](Loads& st, int pos) {
-    // the tiles' rows, as many as are valid (the others arrive as zeros), and their head's powers
-    __amdgpu_buffer_rsrc_t k_at[2], v_at[2], ks_at[2], vs_at[2];
+    __amdgpu_buffer_rsrc_t k_at[2] = {k_all, k_all}, v_at[2] = {v_all, v_all};
+    __amdgpu_buffer_rsrc_t ks_at[2] = {ks_all, ks_all}, vs_at[2] = {vs_all, vs_all};
+    uint32_t at[2], sat[2];  // the tiles' first rows and powers, from the resources' bases
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int p = pos + 16 * t;
-      const uint32_t page = static_cast<uint32_t>(ids.page[t]);
-      const bool ok = page < pages_u32;
-      const int count = __builtin_amdgcn_readfirstlane(ok ? max(0, min(16, end - p)) : 0);
-      st.count[t] = count;
+      const uint32_t page_id = static_cast<uint32_t>(ids.page[t]);
+      const bool ok = page_id < pages_u32;
+      const uint32_t page = ok ? page_id : 0u, slot = static_cast<uint32_t>(p & mask);
+      int count = min(end - p, 16);
+      asm("" : "+s"(count));  // (a clamp would become a vector median)
+      st.count[t] = ok ? max(count, 0) : 0;
       bad |= !ok;
-      const uint32_t slot = static_cast<uint32_t>(p & mask);
-      const int64_t at = static_cast<int64_t>(ok ? page : 0u) * a.c.page_stride + static_cast<int64_t>(slot * es);
-      const int64_t sat = static_cast<int64_t>(ok ? page : 0u) * a.c.scale_page_stride + slot;
-      const int bytes = count * static_cast<int>(es), sbytes = count > 0 ? static_cast<int>(D / kFp4Block * ps - slot) : 0;
-      k_at[t] = buffer_of(k_head + at, bytes);
-      v_at[t] = buffer_of(v_head + at, bytes);
-      ks_at[t] = buffer_of(ks_head + sat, sbytes);
-      vs_at[t] = buffer_of(vs_head + sat, sbytes);
+      if constexpr (kWide) {
+        const int64_t code = static_cast<int64_t>(page) * a.c.page_stride + slot * es;
+        const int64_t power = static_cast<int64_t>(page) * a.c.scale_page_stride + slot;
+        const int bytes = 16 * static_cast<int>(es), sbytes = static_cast<int>(D / kFp4Block * ps - slot);
+        k_at[t] = buffer_of(k_head + code, bytes);
+        v_at[t] = buffer_of(v_head + code, bytes);
+        ks_at[t] = buffer_of(ks_head + power, sbytes);
+        vs_at[t] = buffer_of(vs_head + power, sbytes);
+        at[t] = sat[t] = 0;
+      } else {
+        at[t] = page * static_cast<uint32_t>(a.c.page_stride) + slot * es;
+        sat[t] = page * static_cast<uint32_t>(a.c.scale_page_stride) + slot;
+      }
     }
     ids = fetch(pos + kRound);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if constexpr (D == 64) {
-        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(k_at[t], k_off, 0, 0);
+        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(k_at[t], k_off, at[t], 0);
         st.k[t][0] = x[0];
         st.k[t][1] = x[1];
       } else {
 #pragma unroll
         for (int h = 0; h < D / 128; ++h) {
-          const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(k_at[t], k_off + 16 * h, 0, 0);
+          const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(k_at[t], k_off + 16 * h, at[t], 0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) st.k[t][4 * h + i] = x[i];
         }
       }
 #pragma unroll
-      for (int h = 0; h < Loads::KP; ++h) st.ks[t][h] = __builtin_amdgcn_raw_buffer_load_b8(ks_at[t], ks_off, h * ps, 0);
+      for (int h = 0; h < Loads::KP; ++h) st.ks[t][h] = __builtin_amdgcn_raw_buffer_load_b8(ks_at[t], ks_off, sat[t] + h * ps, 0);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (D == 64) {
-          st.v[t][i][0] = __builtin_amdgcn_raw_buffer_load_b16(v_at[t], v_off, i * es, 0);
+          st.v[t][i][0] = __builtin_amdgcn_raw_buffer_load_b16(v_at[t], v_off, at[t] + i * es, 0);
         } else if constexpr (D == 128) {
-          st.v[t][i][0] = __builtin_amdgcn_raw_buffer_load_b32(v_at[t], v_off, i * es, 0);
+          st.v[t][i][0] = __builtin_amdgcn_raw_buffer_load_b32(v_at[t], v_off, at[t] + i * es, 0);
         } else {
-          const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(v_at[t], v_off, i * es, 0);
+          const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(v_at[t], v_off, at[t] + i * es, 0);
           st.v[t][i][0] = x[0];
           st.v[t][i][1] = x[1];
         }
       }
-      st.vs[t] = __builtin_amdgcn_raw_buffer_load_b32(vs_at[t], vs_off, 0, 0);
+      st.vs[t] = __builtin_amdgcn_raw_buffer_load_b32(vs_at[t], vs_off, sat[t], 0);
     }
   };
 
@@ -225,8 +240,12 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_spli
         const int left = st.count[t] - 4 * r;  // valid positions of this lane's four
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (j >= left) s[t][j] = kNegInf;
-        // (the values' codes are zeros there, but a power of 255 would make them NaN)
+          if (j >= left) {
+            s[t][j] = kNegInf;
+#pragma unroll
+            for (int x = 0; x < Loads::VW; ++x) st.v[t][j][x] = 0u;
+          }
+        // (a power of 255 would make even zeros NaN)
         st.vs[t] = left >= 4 ? st.vs[t] : left <= 0 ? 0u : st.vs[t] & ((1u << (8 * left)) - 1u);
       }
     }
@@ -374,11 +393,12 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_spli
 }
 
 template <int D>
-int launch_fp4_decode(const Fp4DecodeArgs& a, int64_t batch, hipStream_t s) {
+int launch_fp4_decode(const Fp4DecodeArgs& a, int64_t batch, bool wide, hipStream_t s) {
   const int64_t items = cdiv(batch * a.max_splits, kXcds) * kXcds;  // (row, split), with the XCDs' remainder
   if (items * a.hk > INT32_MAX) return MAS_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<uint32_t>(items * a.hk));
-  hipLaunchKernelGGL(fp4_decode_split<D>, grid, dim3(64 * kWaves), 0, s, a);
+  if (wide) hipLaunchKernelGGL((fp4_decode_split<D, true>), grid, dim3(64 * kWaves), 0, s, a);
+  else hipLaunchKernelGGL((fp4_decode_split<D, false>), grid, dim3(64 * kWaves), 0, s, a);
   if (const int st = launch_status(); st != MAS_OK || a.max_splits == 1) return st;  // (no row of several splits)
   hipLaunchKernelGGL((decode_attn_combine<D, fp4_split_len>), dim3(static_cast<uint32_t>(a.hq), static_cast<uint32_t>(batch)),
                      dim3(64), 0, s, a);
@@ -468,9 +488,15 @@ extern "C" int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int
   a.quant_scale_dev = out_scale_dev;
   a.quant_scale_host = out_scale_host;
   a.err = err;
+  // A head's codes reach over the pages before the last one, that page's rows and one row; its powers likewise.
+  const int64_t code_bytes = (num_pages - 1) * page_stride + (page_size - 1) * entry_stride + head_dim / 2;
+  const int64_t power_bytes = (num_pages - 1) * scale_page_stride + head_dim / kFp4Block * page_size;
+  const bool wide = page_stride < 0 || scale_page_stride < 0 || code_bytes > INT32_MAX || power_bytes > INT32_MAX;
+  a.code_bytes = wide ? 0 : static_cast<int>(code_bytes);
+  a.power_bytes = wide ? 0 : static_cast<int>(power_bytes);
   switch (head_dim) {
-    case 64: return launch_fp4_decode<64>(a, batch, stream);
-    case 128: return launch_fp4_decode<128>(a, batch, stream);
-    default: return launch_fp4_decode<256>(a, batch, stream);
+    case 64: return launch_fp4_decode<64>(a, batch, wide, stream);
+    case 128: return launch_fp4_decode<128>(a, batch, wide, stream);
+    default: return launch_fp4_decode<256>(a, batch, wide, stream);
   }
 }
