@@ -22,7 +22,7 @@ from __future__ import annotations
 
 import torch
 
-from . import activation, attention, embedding, fused, norm, page, rope
+from . import activation, attention, embedding, fused, norm, page, rope, step
 from .workloads import (LayerInputs, Shape, StepShape, credited_bytes, layer_credited_bytes, make_layer_inputs,
                         make_step_layout)
 
@@ -129,13 +129,25 @@ class ForwardStep:
     every row's positions), its own stand-ins and norm weights; one residual stream runs through all
     of them. Rows and tokens follow the runner's prepare() (make_step_layout). The workspace is the
     reference's 128 MiB buffer (devstral2.py:35), shared by both attention calls.
+
+    ``kv_format="fp4"`` runs the same step over KV caches held in 4 bits (page.Fp4KVCache, "HND"), planned on the
+    device: first plan_step, from the rows' lengths and a ring of free pages that hands out the layout's own pages
+    (``plan`` then holds the step's index tensors: padding tokens come last, in no row and no slot, where the host's
+    layout gives them a row on a sink page); step 2 is RoPE and the quantizing store, by slots; step 3 the two
+    attentions over the 4-bit cache. Positions lie below the llama-4 interval, where the query scale is 1.
     """
 
     LLAMA_4_BETA = 0.1
     LLAMA_4_ORIGINAL_MAX = 8192
 
-    def __init__(self, shape: StepShape, device: torch.device, seed: int = 0, act_scale: float = 0.05):
+    def __init__(self, shape: StepShape, device: torch.device, seed: int = 0, act_scale: float = 0.05,
+                 kv_format: str = "bf16"):
+        if kv_format not in ("bf16", "fp4"):
+            raise ValueError(f"kv_format must be 'bf16' or 'fp4', got {kv_format!r}")
+        if kv_format == "fp4" and shape.reach > self.LLAMA_4_ORIGINAL_MAX:
+            raise ValueError("a step over a 4-bit cache keeps to positions whose query scale is 1")
         self.shape = shape
+        self.kv_format = kv_format
         ls = shape.layer
         self.device = device
         lay = make_step_layout(shape, seed)
@@ -175,9 +187,17 @@ class ForwardStep:
                 "o_proj": normal(n, ls.hidden),
                 "w_post": normal(ls.hidden, scale=0.1, shift=1.0),
                 "gate_up": normal(n, 2 * ls.inter),
-                "k_cache": k0.clone(), "v_cache": v0.clone(),
             })
+            if kv_format == "bf16":
+                self.layers[-1].update(k_cache=k0.clone(), v_cache=v0.clone())
+            else:
+                cache = page.fp4_kv_cache(lay.pages, shape.page_size, ls.kv_heads, ls.head_dim, device, "HND")
+                page.store_kv_slots_fp4(k0.flatten(0, 1), v0.flatten(0, 1), cache,
+                                        torch.arange(lay.pages * shape.page_size, device=device), "HND")
+                self.layers[-1]["kv"] = cache
         del k0, v0
+        if kv_format == "fp4":
+            self._plan_inputs(lay)
         self.final_in = normal(n, ls.hidden)               # the last down_proj output
         self.final_weight = normal(ls.hidden, scale=0.1, shift=1.0)
         self.norm_out = torch.empty(n, ls.hidden, dtype=torch.float8_e4m3fn, device=device)
@@ -186,6 +206,32 @@ class ForwardStep:
         self.embed_table = normal(ls.vocab, ls.hidden)
         cpu = torch.Generator().manual_seed(seed)
         self.ids = torch.randint(0, ls.vocab, (n,), generator=cpu).to(device)
+
+    def _plan_inputs(self, lay) -> None:
+        """What plan_step makes the step from: each row's cached and new positions, block tables that end with the
+        cached ones, and a ring with the pages that the layout has after them, in row order."""
+        shape, d, ps = self.shape, lay.num_decodes, self.shape.page_size
+        rows = self.block_tables.shape[0]
+        new = torch.zeros(rows, dtype=torch.int32)
+        new[:d] = 1
+        for j, (q, _) in enumerate(shape.prompts):
+            new[d + j] = q
+        cached = torch.where(new > 0, lay.seq_lens - new, torch.zeros_like(new))
+        tables, ring = torch.full_like(lay.block_tables, -1), []
+        for r in range(rows):
+            if new[r] > 0:
+                have, need = -(-int(cached[r]) // ps), -(-int(cached[r] + new[r]) // ps)
+                tables[r, :have] = lay.block_tables[r, :have]
+                ring += lay.block_tables[r, have:need].tolist()
+        self.new_lens, self.cached_lens = new.to(self.device), cached.to(self.device)
+        self.block_tables = tables.to(self.device)
+        self.free_pages = torch.tensor(ring + [lay.pages - 1], dtype=torch.int32, device=self.device)
+        self.free_range = torch.tensor([0, len(ring)], device=self.device)
+        self.plan = step.step_tables(rows, lay.num_tokens, self.device)
+
+    def run_plan(self) -> None:
+        step.plan_step(self.new_lens, self.cached_lens, self.block_tables, self.free_pages, self.free_range,
+                       self.shape.page_size, self.num_tokens, out=self.plan)
 
     def views(self, layer: dict):
         """q [tokens, Hq, D], k [tokens, Hk * D] and v [tokens, Hk, D]: column views of the qkv stand-in
@@ -203,6 +249,10 @@ class ForwardStep:
     def run_rope_append(self, layer: dict) -> None:
         ls = self.shape.layer
         q, k, v = self.views(layer)
+        if self.kv_format == "fp4":
+            rope.apply_rope_with_cos_sin_cache_inplace(self.plan.positions, q, k, ls.head_dim, self.table, True)
+            page.store_kv_slots_fp4(k, v, layer["kv"], self.plan.slot_mapping, "HND")
+            return
         fused.apply_rope_and_append_paged_kv_cache(
             self.positions, q, k, v, ls.head_dim, self.table, True, self.batch_indices,
             (layer["k_cache"], layer["v_cache"]), self.kv_indices, self.kv_indptr, None, "NHD",
@@ -213,6 +263,11 @@ class ForwardStep:
         if d == 0:
             return
         q = self.views(layer)[0].unflatten(-1, (ls.q_heads, ls.head_dim))
+        if self.kv_format == "fp4":
+            attention.batch_decode_with_fp4_kv_cache(
+                q[:d], layer["kv"], self.workspace, self.block_tables[:d], self.plan.seq_lens[:d], self.max_kv_len,
+                self.scale, 1.0, out=self.attn_out[:d], kv_layout="HND", out_quant_scale=self.act_scale)
+            return
         attention.trtllm_batch_decode_with_kv_cache(
             q[:d], (layer["k_cache"], layer["v_cache"]), self.workspace, self.block_tables[:d], self.seq_lens[:d],
             self.max_kv_len, self.scale, 1.0, out=self.attn_out[:d], out_quant_scale=self.act_scale)
@@ -222,6 +277,12 @@ class ForwardStep:
         if self.num_prefills == 0:
             return
         q = self.views(layer)[0].unflatten(-1, (ls.q_heads, ls.head_dim))
+        if self.kv_format == "fp4":
+            attention.batch_context_with_fp4_kv_cache(
+                q, layer["kv"], self.workspace, self.block_tables[d:], self.plan.seq_lens[d:], self.max_q_len,
+                self.max_kv_len, self.scale, 1.0, self.num_prefills, self.plan.cu_seqlens_q[d:], None,
+                out=self.attn_out, kv_layout="HND", out_quant_scale=self.act_scale)
+            return
         attention.trtllm_batch_context_with_kv_cache(
             q[d:], (layer["k_cache"], layer["v_cache"]), self.workspace, self.block_tables[d:], self.seq_lens[d:],
             self.max_q_len, self.max_kv_len, self.scale, 1.0, self.num_prefills, self.cu_seqlens_q, None,
@@ -244,6 +305,8 @@ class ForwardStep:
     LAYER_OPS = ("norm_in", "rope_append", "decode_attention", "context_attention", "norm_post", "silu")
 
     def run(self) -> None:
+        if self.kv_format == "fp4":
+            self.run_plan()
         self.run_embedding()
         for layer in self.layers:
             for op in self.LAYER_OPS:
