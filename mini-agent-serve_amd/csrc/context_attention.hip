@@ -864,11 +864,30 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
     }
     return x;
   };
+  // A value that is no finite bf16 (NaN, or past the largest one) must not meet a weight of zero in the MFMAs: the
+  // tokens before it would get 0 * NaN. Its element is staged as zero, and nan_from[dim] holds the first position of
+  // one: the tokens from there on get NaN in that dim after the last tile (fp4_end). nan_from[D] is the least of them.
+  __shared__ int nan_from[kFp4 ? D + 1 : 1];
   // Piece i (of four, 8 elements each) of a chunk into its place in a tile buffer. Values take the pieces in an
   // order turned by the row (fp4_turn), so that the 16 lanes of a store's phase, four rows of four chunks, hit all
   // 16 slots of the banks; a key row's swizzle alone does that.
-  auto fp4_turn = [&](Fp4Regs& x, bool values) {
+  auto fp4_turn = [&](Fp4Regs& x, bool values, int tile) {
     if constexpr (kFp4) {
+      if (values && x.ok && x.power >= 253u) {  // 2^126: codes of 4 and 6 pass bf16's largest; 2^127: of 2 and on
+        const uint32_t least = x.power == 255u ? 0u : x.power == 254u ? 4u : 6u;
+#pragma unroll 1
+        for (int e = 0; e < kFp4Block; ++e) {  // (the words take turns in the first place)
+          uint32_t w = x.w[0] >> 4 | x.w[0] << 28;
+          if ((x.w[0] & 7u) >= least) {
+            w &= 0x0fffffffu;
+            atomicMin(&nan_from[kFp4Block * f_chunk + e], tile * kTileP + f_row);
+            atomicMin(&nan_from[D], tile * kTileP + f_row);
+          }
+          x.w[0] = w;
+          if ((e & 7) == 7) x.w = u32x4{x.w[1], x.w[2], x.w[3], w};
+        }
+        if (x.power == 255u) x.power = 0u;
+      }
       if (!x.ok) {  // past the sequence, or on a bad page: zeros
         x.w = u32x4{0u, 0u, 0u, 0u};
         x.power = 0u;
@@ -887,8 +906,8 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
       *reinterpret_cast<u32x4*>(dst + ((values ? f_value_at : f_key_at) ^ 8 * i)) =
           fp4x8_decode(x.w[i], __uint_as_float(x.power << 23));
   };
-  auto fp4_stage = [&](Fp4Regs& x, uint16_t* dst, bool values) {
-    fp4_turn(x, values);
+  auto fp4_stage = [&](Fp4Regs& x, uint16_t* dst, bool values, int tile) {
+    fp4_turn(x, values, tile);
 #pragma unroll
     for (int i = 0; i < 4; ++i) fp4_put(x, dst, values, i);
   };
@@ -1059,6 +1078,8 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
   const auto f_limit = [&](int tile) { return tile < it_end ? kv_len : 0; };
   if (it_begin < it_end) {
     if constexpr (kFp4) {
+      for (int i = tid; i <= D; i += kCtxThreads) nan_from[i] = INT32_MAX;
+      __syncthreads();
       const Fp4Pages p0 = fp4_find(it_begin * kTileP, true, kv_len);
       const Fp4Pages p1 = fp4_find((it_begin + 1) * kTileP, true, f_limit(it_begin + 1));
       f_ahead = fp4_find((it_begin + 2) * kTileP, true, f_limit(it_begin + 2));
@@ -1066,18 +1087,18 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
         Fp4Regs k0 = fp4_issue(p0, false), v0 = fp4_issue(p0, true), k1 = fp4_issue(p1, false);
         f_k = fp4_issue(f_ahead, false);
         f_v = fp4_issue(p1, true);
-        fp4_stage(k0, klds(0), false);
-        fp4_stage(v0, vlds(0), true);
-        fp4_stage(k1, klds(1), false);
+        fp4_stage(k0, klds(0), false, it_begin);
+        fp4_stage(v0, vlds(0), true, it_begin);
+        fp4_stage(k1, klds(1), false, it_begin + 1);
       } else if (f_role == 0) {
         Fp4Regs k0 = fp4_issue(p0, false), k1 = fp4_issue(p1, false);
         f_k = fp4_issue(f_ahead, false);
-        fp4_stage(k0, klds(0), false);
-        fp4_stage(k1, klds(1), false);
+        fp4_stage(k0, klds(0), false, it_begin);
+        fp4_stage(k1, klds(1), false, it_begin + 1);
       } else if (f_role == 1) {
         Fp4Regs v0 = fp4_issue(p0, true);
         f_k = fp4_issue(p1, true);
-        fp4_stage(v0, vlds(0), true);
+        fp4_stage(v0, vlds(0), true, it_begin);
       }
       page_chunk = chunk_of((it_begin + (f_role == 0 ? 3 : 2)) * kTileP);
       page_ids = load_page_ids(page_chunk);
@@ -1133,12 +1154,12 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
       if constexpr (kBoth) {
         f_pages = f_ahead;
         f_ahead = fp4_find((it + 3) * kTileP, false, f_limit(it + 3));
-        fp4_turn(f_v, true);
-        fp4_turn(f_k, false);
+        fp4_turn(f_v, true, it + 1);
+        fp4_turn(f_k, false, it + 2);
       } else if (f_role < 2) {
         const int next = f_role == 0 ? it + 3 : it + 2;
         f_ahead = fp4_find(next * kTileP, false, f_limit(next));
-        fp4_turn(f_k, f_role == 1);
+        fp4_turn(f_k, f_role == 1, f_role == 0 ? it + 2 : it + 1);
       }
     } else if constexpr (kDirect) {
       __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
@@ -1226,6 +1247,16 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
   if (len_bad && tid == 0 && blockIdx.x == 0 && tile_idx == 0) report(a.err, MAS_ERRBIT_POSITION);
 
   if (!wave_live) return;
+  if constexpr (kFp4) {  // fp4_end: the last tile's barrier is behind every nan_from
+    if (it_begin < it_end && nan_from[D] != INT32_MAX) {
+      const int at = shift + tok + n;  // this lane's token's position
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (nan_from[32 * db + 8 * (j >> 2) + 4 * hf + (j & 3)] <= at) acc[db][j] = __builtin_nanf("");
+    }
+  }
   l_run += __shfl_xor(l_run, 32);  // the row's sum: both halves' shares
   // ---- Output. A lane holds 4-column pieces of its token's row, so stores straight from the registers
   // would touch 32 rows per instruction: they took 2.3 us of a workgroup's 36 at 4 x 2048 tokens of 32

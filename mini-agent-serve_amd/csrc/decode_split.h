@@ -223,57 +223,6 @@ __global__ __launch_bounds__(64) void decode_attn_combine(DecodeArgs a) {
 int64_t decode_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t head_dim, int64_t splits) {
   return batch * num_q_heads * (splits > 0 ? splits : 1) * (head_dim + 2) * 4;
 }
-// Returned by decode_attention when even one split per row does not fit the workspace.
-constexpr int kWorkspaceTooSmall = -1000;
-
-// How a launch cuts its rows: the longest split, the splits of the longest row (the grid's size), and the
-// splits wanted per row in small grids.
-struct DecodeSplits {
-  int64_t split_len, splits;
-  int row_target;
-};
-
-// `cap`: the block table's reach in positions. Returns kWorkspaceTooSmall, or an error code.
-int decode_splits(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t cap,
-                  const void* workspace, int64_t workspace_bytes, DecodeSplits* out) {
-  // The smallest split (most parallelism) whose partials fit the workspace, with at most
-  // kMaxSplitItems (row, kv head, split) work items and kMaxRowSplits splits per row: past those,
-  // more splits only add per-split overhead, partials and combine passes (64 rows x 8 kv heads x
-  // 128 splits of 256 positions: 804 us per call, with 4 chunks per split 738 us; 8 rows x 8 kv
-  // heads x 128 splits: 124 us, with 2 chunks per split 117 us).
-  const int64_t chunks = cdiv(cap, kChunk);
-  constexpr int64_t kMaxSplitItems = 16384, kMaxRowSplits = 64;
-  int64_t per_split = 1;
-  while (per_split < chunks &&
-         (decode_workspace_bytes(batch, num_q_heads, head_dim, cdiv(chunks, per_split)) > workspace_bytes ||
-          cdiv(chunks, per_split) > kMaxRowSplits || batch * num_kv_heads * cdiv(chunks, per_split) > kMaxSplitItems))
-    per_split *= 2;
-  if (per_split > chunks) per_split = chunks > 0 ? chunks : 1;
-  if (workspace == nullptr) return MAS_ERR_INVALID_VALUE;
-  if (decode_workspace_bytes(batch, num_q_heads, head_dim, cdiv(chunks, per_split)) > workspace_bytes)
-    return kWorkspaceTooSmall;
-  int64_t split_len = per_split * kChunk;
-  // Small grids: splits of 128 or 64 positions while the grid holds fewer work items than the GPU
-  // has SIMDs, at most 128 splits per row and within the workspace. A split of 256 positions is 8
-  // dependent steps; with few wavefronts those steps' latencies, not bandwidth, set the time (on
-  // MI355X: 16 rows of up to 512 positions 15.8 -> 10.1 us, one row of up to 4096 14.8 -> 9.6 us;
-  // at one item per SIMD and more, shorter splits lost: 64 rows of up to 512, 22.0 -> 23.5 us).
-  int cus = 0;
-  if (const int st = device_cu_count(&cus); st != MAS_OK) return st;
-  if (per_split == 1 && cap > 0) {
-    const int64_t simds = static_cast<int64_t>(cus) * 4;
-    while (split_len > 64 && batch * num_kv_heads * cdiv(cap, split_len) < simds &&
-           cdiv(cap, split_len / 2) <= 2 * kMaxRowSplits &&
-           decode_workspace_bytes(batch, num_q_heads, head_dim, cdiv(cap, split_len / 2)) <= workspace_bytes)
-      split_len /= 2;
-  }
-  const int64_t splits = cap > 0 ? cdiv(cap, split_len) : 1;
-  out->split_len = split_len;
-  out->splits = splits;
-  out->row_target =
-      static_cast<int>(std::max<int64_t>(1, static_cast<int64_t>(cus) * 4 / std::max<int64_t>(1, batch * num_kv_heads)));
-  return MAS_OK;
-}
 
 }  // namespace
 }  // namespace mas

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from conftest import bits
-from fp4_common import P_BF16, Cache, check, random_rows
+from fp4_common import P_BF16, Cache, check, random_rows, tolerance
 from oracle import fp4
 
 pytestmark = pytest.mark.gpu
@@ -132,6 +132,49 @@ def test_a_nan_that_counts_shows(mas, dev):
     cache.tensors[2][int(tables[0, 2]), 0, 1, 8] = 255
     out = _run(mas, dev, cache, q, tables, lens, cu, 0.1).cpu()
     assert bool(out[:40].isfinite().all()) and bool(out[40:].isnan().all())
+
+
+@pytest.mark.parametrize("hq,hk,dim,ws_bytes", [(4, 1, 128, 0), (8, 1, 128, 0), (4, 1, 64, 0), (12, 1, 64, 0), (4, 1, 128, 8 << 20)])
+def test_values_that_are_no_numbers_reach_only_the_tokens_after_them(mas, dev, hq, hk, dim, ws_bytes):
+    """NaN value blocks, and values past bf16's largest number, at positions inside the prompt: the tokens before them,
+    whose weight there is none, are as if they were not there; the tokens from them on are NaN in those elements."""
+    rows = [(150, 900 if ws_bytes else 300), (40, 40)]
+    cache, q, tables, lens, cu = _case(27, hq, hk, dim, 16, "HND", rows)
+    first, large = {}, {}                            # (row, element): its first position that is no number
+
+    def spoil(r, p, element, power, code):
+        page, slot = int(tables[r, p // 16]), p % 16
+        cache.tensors[3][page, 0, element // 32, slot] = power
+        row = cache.tensors[1][page, 0, slot]
+        row[16 * (element // 32):16 * (element // 32) + 16] = 0x11     # 1/2: finite at any power below 255
+        row[element // 2] = code | code << 4
+        cols = range(element // 32 * 32, element // 32 * 32 + 32) if power == 255 else (element & ~1, element | 1)
+        for c in cols:
+            first[r, c] = min(p, first.get((r, c), p))
+        large[r, p, element // 32] = power
+
+    n = lens[0]
+    spoil(0, n - 150 + 33, 5, 255, 0)
+    spoil(0, n - 150 + 97, 7, 255, 0)
+    spoil(0, n - 2, 40, 254, 4)                      # 2 * 2^127
+    spoil(0, n - 70, 62, 253, 14)                    # -4 * 2^126
+    spoil(1, 39, 33, 254, 7)
+    out = _run(mas, dev, cache, q, tables, lens, cu, 2.0 ** -10, ws_bytes=ws_bytes).float().cpu().numpy()
+    values = cache.v.copy()
+    spoiled = np.zeros_like(out, dtype=bool)
+    for (r, p, block), power in large.items():
+        page, slot = int(tables[r, p // 16]), p % 16
+        values[page, slot, 0, 32 * block:32 * block + 32] = 0.0
+        t = int(cu[r]) + p - (lens[r] - rows[r][0])
+        spoiled[t:int(cu[r + 1]), :, 32 * block:32 * block + 32] = True
+    want = fp4.context_attention(bits(q), cache.k, values, tables.numpy(), lens, cu, 2.0 ** -10)
+    ok = ~spoiled
+    allowed = tolerance(*want, max(lens), P_BF16)
+    assert np.isfinite(out[ok]).all() and (np.abs(out - want[0])[ok] <= allowed[ok]).all()
+    no_number = np.zeros_like(spoiled)
+    for (r, c), p in first.items():
+        no_number[int(cu[r]) + p - (lens[r] - rows[r][0]):int(cu[r + 1]), :, c] = True
+    assert np.isnan(out[no_number]).all() and np.isfinite(out[~no_number]).all()
 
 
 @pytest.mark.parametrize("scale,size", [(0.1, 2.0 ** 50), (0.1, 2.0 ** -50), (3.0, 4.0)])
