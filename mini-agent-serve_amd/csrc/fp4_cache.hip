@@ -219,7 +219,8 @@ int check_rows(Fp4Args& a, int64_t num_heads, int64_t head_dim, bool* empty) {
   a.vec_per_head = static_cast<int>(head_dim / 8);
   a.vec_per_row = static_cast<int>(num_heads * head_dim / 8);
   a.parts = static_cast<int>(cdiv(a.vec_per_row, kWave));
-  return cdiv(a.rows, tokens_per_wave(a.rows, a.parts)) * 2 * a.parts > INT32_MAX ? MAS_ERR_UNSUPPORTED : MAS_OK;
+  // (a grid is below 2^32 threads)
+  return cdiv(a.rows, tokens_per_wave(a.rows, a.parts)) * 2 * a.parts * kWave > UINT32_MAX ? MAS_ERR_UNSUPPORTED : MAS_OK;
 }
 
 enum class Move { kAppend, kStore, kLoad };

@@ -42,6 +42,7 @@ constexpr int kStep = 32;                    // positions a wavefront takes at a
 constexpr int kRound = kWaves * kStep;       // and a workgroup
 constexpr int kMaxSplitLen = 1024;           // positions per split, at most, while max_splits reach
 constexpr int kMaxSplits = 128;
+constexpr int64_t kMaxItems = int64_t{1} << 23;  // workgroups of a launch, at most (a grid is below 2^32 threads)
 
 // A row's split length: its share of row_target splits, in whole rounds, at most kMaxSplitLen; and such that its splits
 // fit the grid and the workspace.
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_spli
       if constexpr (kWide) {
         const int64_t code = static_cast<int64_t>(page) * a.c.page_stride + slot * es;
         const int64_t power = static_cast<int64_t>(page) * a.c.scale_page_stride + slot;
-        const int bytes = 16 * static_cast<int>(es), sbytes = static_cast<int>(D / kFp4Block * ps - slot);
+        const int bytes = 15 * static_cast<int>(es) + D / 2, sbytes = static_cast<int>(D / kFp4Block * ps - slot);
         k_at[t] = buffer_of(k_head + code, bytes);
         v_at[t] = buffer_of(v_head + code, bytes);
         ks_at[t] = buffer_of(ks_head + power, sbytes);
@@ -395,7 +396,6 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_spli
 template <int D>
 int launch_fp4_decode(const Fp4DecodeArgs& a, int64_t batch, bool wide, hipStream_t s) {
   const int64_t items = cdiv(batch * a.max_splits, kXcds) * kXcds;  // (row, split), with the XCDs' remainder
-  if (items * a.hk > INT32_MAX) return MAS_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<uint32_t>(items * a.hk));
   if (wide) hipLaunchKernelGGL((fp4_decode_split<D, true>), grid, dim3(64 * kWaves), 0, s, a);
   else hipLaunchKernelGGL((fp4_decode_split<D, false>), grid, dim3(64 * kWaves), 0, s, a);
@@ -441,8 +441,8 @@ extern "C" int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int
   if (group > 16 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return MAS_ERR_UNSUPPORTED;
   const int64_t cap = max_blocks * page_size;
   // (a page's rows are addressed with 32-bit byte offsets)
-  if (cap > (int64_t{1} << 30) || batch > 65535 || num_kv_heads > 65535 || num_q_heads > 65535 || entry_stride < 0 ||
-      page_size * entry_stride > INT32_MAX)
+  if (cap > (int64_t{1} << 30) || batch > 65535 || num_kv_heads > 65535 || num_q_heads > 65535 ||
+      batch * num_kv_heads > kMaxItems || entry_stride < 0 || page_size * entry_stride > INT32_MAX)
     return MAS_ERR_UNSUPPORTED;
   if (out == nullptr || q == nullptr || seq_lens == nullptr ||
       (cap > 0 && (block_tables == nullptr || num_pages == 0)))
@@ -460,7 +460,8 @@ extern "C" int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int
   const int64_t held = workspace_bytes / decode_workspace_bytes(batch, num_q_heads, head_dim, 1);
   if (held < 1) return MAS_ERR_INVALID_VALUE;
   const int64_t splits = std::max<int64_t>(
-      1, std::min({std::max(std::min(target, cdiv(cap, kRound)), cdiv(cap, kMaxSplitLen)), int64_t{kMaxSplits}, held}));
+      1, std::min({std::max(std::min(target, cdiv(cap, kRound)), cdiv(cap, kMaxSplitLen)), int64_t{kMaxSplits}, held,
+                   kMaxItems / (batch * num_kv_heads)}));
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_stride;
   a.q_head_stride = q_head_stride;

@@ -165,17 +165,17 @@ def test_c_entry_points_refuse(mas):
     for change, status in ((dict(ps=8), -2), (dict(ps=24), -2), (dict(ps=0), -1), (dict(dim=48), -2), (dict(k=None), -1),
                            (dict(k=P + 8), -3), (dict(stride=40), -3), (dict(scale=P + 2), -3), (dict(key=P + 4), -3),
                            (dict(key=None), -1), (dict(slots=None), -1), (dict(rows=-1), -1), (dict(pages=-1), -1),
-                           (dict(rows=1 << 40), -2)):
+                           (dict(rows=1 << 40), -2), (dict(rows=1 << 27), -2)):
         assert store(**change) == status, change
 
-    def decode(ps=16, dim=128, hq=8, hk=2, out=P, ws=P, ws_bytes=1 << 20, blocks=4, pages=4, tables=P, entry=128, fp8=0, quant=0.0):
+    def decode(ps=16, dim=128, hq=8, hk=2, out=P, ws=P, ws_bytes=1 << 20, blocks=4, pages=4, tables=P, entry=128, fp8=0, quant=0.0, batch=3):
         return lib.mas_paged_decode_attention_fp4(out, 1024, 128, P, 1024, 128, P, P, 4096, entry, 64, P, P, 128, 64, pages,
-                                                  ps, tables, 4, blocks, P, 3, hq, hk, dim, 0.1, 1.0, fp8, None, quant, ws,
+                                                  ps, tables, 4, blocks, P, batch, hq, hk, dim, 0.1, 1.0, fp8, None, quant, ws,
                                                   ws_bytes, None, None)
     for change, status in ((dict(ps=8), -2), (dict(dim=96), -2), (dict(hq=34), -2), (dict(hq=7), -1), (dict(hk=0), -1),
                            (dict(out=None), -1), (dict(out=P + 2), -3), (dict(ws=None), -1), (dict(ws=P + 4), -3),
                            (dict(pages=0), -1), (dict(tables=None), -1), (dict(entry=1 << 30), -2), (dict(fp8=1), -1),
-                           (dict(blocks=1 << 40), -2)):
+                           (dict(blocks=1 << 40), -2), (dict(batch=65536), -2), (dict(batch=65535, hq=200, hk=200), -2)):
         assert decode(**change) == status, change
     assert decode(hq=0) == 0 and decode(ws_bytes=16) in (-1, -4)   # (-4: no GPU to ask for its size)
 

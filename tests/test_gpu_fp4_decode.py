@@ -205,3 +205,36 @@ def test_pages_far_into_a_large_cache(mas, dev):
         q.to(dev), c, torch.empty(1 << 20, dtype=torch.uint8, device=dev), (tables + pages - 4).to(torch.int32).to(dev),
         torch.tensor(lens, dtype=torch.int32, device=dev), 0, 0.1, 1.0, kv_layout="HND")
     check(out, fp4.decode_attention(bits(q), few.k, few.v, tables.numpy(), lens, 0.1), 60, P_TWO_TERMS)
+
+
+@pytest.mark.parametrize("dim,pages,layout", [(64, 5 << 20, "NHD"), (256, 2 << 20, "HND")])
+def test_other_head_dims_in_a_large_cache(mas, dev, dim, pages, layout):
+    few = Cache(15, 16, 16, 1, dim, layout)
+    c = mas.page.fp4_kv_cache(pages, 16, 1, dim, dev, layout)
+    for t, s in zip(c, few.tensors):
+        t[-16:] = s.to(dev)
+    q, lens = random_rows(16, 2, 5, dim), [250, 128]
+    tables = torch.stack([torch.randperm(16, generator=torch.Generator().manual_seed(i)) for i in range(2)])
+    out = mas.attention.batch_decode_with_fp4_kv_cache(
+        q.to(dev), c, torch.empty(1 << 20, dtype=torch.uint8, device=dev), (tables + pages - 16).to(torch.int32).to(dev),
+        torch.tensor(lens, dtype=torch.int32, device=dev), 0, 0.1, 1.0, kv_layout=layout)
+    check(out, fp4.decode_attention(bits(q), few.k, few.v, tables.numpy(), lens, 0.1), 250, P_TWO_TERMS)
+
+
+def test_as_many_rows_as_a_call_takes(mas, dev):
+    """65535 rows of 8 kv heads under a table of 40 pages of 1024: more (row, head, 1024 positions) than a grid holds, so
+    the splits get longer; rows of all lengths, some as long as the table."""
+    rows, ps, width, dim = 65535, 1024, 40, 64
+    cache = Cache(17, 2, ps, 8, dim, "HND")
+    g = torch.Generator().manual_seed(18)
+    lens = torch.randint(0, 50, (rows,), generator=g).to(torch.int32)
+    tables = torch.randint(0, 2, (rows, width), generator=g).to(torch.int32)
+    some = [0, 1, 777, 32768, 65533, 65534]
+    for r, n in zip(some, (width * ps, 1, 5000, 20481, 0, 16 * ps + 1)):
+        lens[r] = n
+    q = random_rows(19, rows, 8, dim)
+    out = _run(mas, dev, cache, q, tables, lens, 0.1, ws_bytes=6 << 30)
+    some += list(range(2000, 2040))
+    want = fp4.decode_attention(bits(q[some]), cache.k, cache.v, tables[some].numpy(), lens[some].tolist(), 0.1)
+    check(out[some], want, width * ps, P_TWO_TERMS)
+    assert bool(out.isfinite().all())
