@@ -373,7 +373,7 @@ int64_t mas_paged_context_attention_workspace_bytes(int64_t num_rows, int64_t ma
  * mas_append_paged_kv_cache_bf16. For each block, s is the smallest byte under which max |x| < 7 * 2^(s - 127)
  * (255 where the block holds a NaN or an infinity, its codes then 0), and each code the nearest one to
  * x / 2^(s - 127), ties to the even code: off by at most half a step. The bits follow from the inputs alone.
- * Duplicate destinations are allowed (what they hold then may mix the writers' blocks).
+ * Duplicate destinations are allowed, but a block may then hold the codes of one row and the power of another.
  */
 int mas_append_paged_kv_cache_fp4(void* k_cache, void* v_cache, int64_t page_stride, int64_t entry_stride,
                                   int64_t head_stride, void* k_scale, void* v_scale, int64_t scale_page_stride,

@@ -16,7 +16,6 @@
 namespace mas {
 namespace {
 
-
 struct Fp4Args : Fp4Cache {
   // the tokens' rows: sources of the store, destinations of the load
   uint16_t* key;
@@ -48,7 +47,6 @@ template <int kCtrl>
 __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, 0xf, 0xf, false));
 }
-
 
 // Where token t's row lies: byte offsets of its codes and powers, less the head's and the block's. Each lane resolves
 // one token (lane % kTokens), so a wavefront's four take one chain of dependent loads (resolved in turn, with scalar loads,

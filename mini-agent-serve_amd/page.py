@@ -278,7 +278,8 @@ def append_paged_kv_cache_fp4(append_key: torch.Tensor, append_value: torch.Tens
 
     Each block of 32 elements gets the smallest power of two (of at least 2^-127) under which its largest element
     lies below 7, and each element the nearest e2m1 code, ties to the even one: the bits follow from the row
-    alone. A block that holds a NaN or an infinity stands for NaN throughout.
+    alone. A block that holds a NaN or an infinity stands for NaN throughout. Two tokens of one call must not share a
+    destination: a block could keep the codes of one and the power of the other.
     """
     if torch.compiler.is_compiling():
         torch.ops.mas.append_paged_kv_cache_fp4(append_key, append_value, batch_indices, positions, *kv_cache,
@@ -314,7 +315,8 @@ def _slots_fp4(entry: str, key, value, kv_cache, slot_mapping, kv_layout: str, e
 def store_kv_slots_fp4(key: torch.Tensor, value: torch.Tensor, kv_cache, slot_mapping: torch.Tensor,
                        kv_layout: str = "NHD", *, error_flags: torch.Tensor | None = None) -> None:
     """Slot-mapping form of ``append_paged_kv_cache_fp4``: token t goes to page ``slot // page_size``, entry
-    ``slot % page_size`` with ``slot = slot_mapping[t]`` (int64); a negative slot is skipped."""
+    ``slot % page_size`` with ``slot = slot_mapping[t]`` (int64); a negative slot is skipped, and no
+    slot is named twice."""
     if torch.compiler.is_compiling():
         torch.ops.mas.store_kv_slots_fp4(key, value, *kv_cache, slot_mapping, kv_layout, error_flags)
         return
