@@ -177,7 +177,11 @@ constexpr int kPagesLane = 0, kPagesTile = 2;
 // kPagesMulti8 + i: pages of 8 << i slots (i < 3)
 constexpr int kPagesMulti8 = 4, kPagesMulti16 = 5, kPagesMulti32 = 6;
 //   kPagesFp4   - the 4-bit cache (pages of at least 16 slots): a lane loads 32 codes of a row and their power,
-//                 and decodes them to bf16 on the way into LDS, a tile after it loaded them.
+//                 and decodes them to bf16 on the way into LDS, a tile after it loaded them: one barrier per tile, the
+//                 products those of the bf16 cache. About 115 vector instructions per tile and wavefront beside 560:
+//                 4 x 2048 tokens 156 us (151 over the bf16 cache), 4 x 4096 of 96 heads 1585 (1596, 1041 TFLOP/s), 128
+//                 after 4096 26.7 (25.6). A piece's decode and store go with one score MFMA and one of P.V; all four of
+//                 them at every second pair or fenced there were even or slower (6 ragged prompts 218 -> 220, 224 us).
 constexpr int kPagesFp4 = 8;
 template <int kPages>
 using ContextArgsOf = std::conditional_t<kPages == kPagesFp4, Fp4ContextArgs, ContextArgs>;
@@ -1040,9 +1044,10 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
                        const f32x16& cur, bool second, bf16x8 (&pb_cur)[2], auto&& load) {
     f32x16 sn{};
     int key_at = key_at0, value_at = value_at0;
-    // kPagesLane with four wavefronts, a tile in registers besides: the copies keep the compiler from holding
-    // all 12 read addresses over the loop (2 x 64 tokens after 3000, 4-slot pages, 28.5 -> 26.8 us; 500 after
-    // 500 32.9 -> 30.3 us).
+    // kPagesLane and kPagesFp4 with four wavefronts, a tile in registers besides: the copies keep the compiler from
+    // holding all 12 read addresses over the loop (2 x 64 tokens after 3000, 4-slot pages, 28.5 -> 26.8 us; 500 after
+    // 500 32.9 -> 30.3 us; over the 4-bit cache 4 x 2048 tokens 180 -> 165 us, 6 ragged prompts 249 -> 228; with eight
+    // wavefronts 4 x 4096 of 96 heads 1609 without, 1674 with them).
     if constexpr (!kDirect && kWaves == 4) asm volatile("" : "+v"(key_at), "+v"(value_at));
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
