@@ -15,6 +15,8 @@
 // One thread per token, and every workgroup sums the rows' tokens and pages itself, 256 rows at a time (a row
 // per thread, both sums in one pass of wavefront scans), until its own tokens are covered: no workgroup
 // waits for another, and one launch does it. What bounds it: the latencies of the lengths, the page and the stores.
+#include <type_traits>
+
 #include "device.h"
 
 namespace mas {
@@ -39,25 +41,30 @@ struct StepArgs {
   int64_t ring;
   const int64_t* range;
   int64_t page_size, num_tokens;
+  int log2_page;  // -1: page_size is no power of two
   uint32_t* err;
 };
 
-__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int64_t o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
-}
-__device__ __forceinline__ int64_t wave_max64(int64_t v) {
-#pragma unroll
-  for (int d = kWave / 2; d > 0; d /= 2) v = max(v, static_cast<int64_t>(__shfl_xor(v, d)));
-  return v;
+// Sums stop at 2^32 - 1, which is more than any count of tokens or pages that is served.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+// Inclusive scan over the wavefront: by DPP within rows of 16 lanes, then the rows' totals.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {
+  const auto from = [](uint32_t x, auto ctrl) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v = add_sat(v, from(v, std::integral_constant<int, 0x111>{}));  // row_shr 1, 2, 4, 8
+  v = add_sat(v, from(v, std::integral_constant<int, 0x112>{}));
+  v = add_sat(v, from(v, std::integral_constant<int, 0x114>{}));
+  v = add_sat(v, from(v, std::integral_constant<int, 0x118>{}));
+  const auto total = [&](int l) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l)); };
+  const uint32_t r0 = total(15), r1 = add_sat(r0, total(31)), r2 = add_sat(r1, total(47));
+  return add_sat(v, lane < 16 ? 0u : lane < 32 ? r0 : lane < 48 ? r1 : r2);
 }
 
 __global__ __launch_bounds__(kPlanBlock) void plan_step(StepArgs a) {
-  __shared__ int64_t sums[2][kPlanWaves], tops[2][kPlanWaves];
+  __shared__ uint32_t sums[2][2][kPlanWaves];            // (256 rows' parity) the wavefronts' tokens and pages
+  __shared__ uint32_t tops[2][kPlanWaves];               // what they serve of them
+  __shared__ int all[kPlanWaves];                        // whether that is all
   __shared__ int ends[kPlanBlock];                       // token past the row's last one
   __shared__ int row_new[kPlanBlock], row_cached[kPlanBlock], row_page[kPlanBlock];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
@@ -65,66 +72,81 @@ __global__ __launch_bounds__(kPlanBlock) void plan_step(StepArgs a) {
   const int64_t last_t = min(static_cast<int64_t>(blockIdx.x + 1) * kPlanBlock, a.num_tokens);
   const bool writer = blockIdx.x == 0;  // of the rows' outputs
   const int64_t head = a.range[0], tail = a.range[1];
-  const int64_t avail = head < 0 || tail < head ? 0 : min(tail - head, a.ring);
-  const int64_t head_at = a.ring > 0 && head >= 0 ? head % a.ring : 0;
+  const uint32_t avail = static_cast<uint32_t>(head < 0 || tail < head ? 0 : min(tail - head, a.ring));
+  const uint32_t most = static_cast<uint32_t>(a.num_tokens);
+  // (a 64-bit remainder takes a few hundred cycles)
+  const int64_t head_at = a.ring <= 0 || head < 0 ? 0
+                          : head <= UINT32_MAX    ? static_cast<uint32_t>(head) % static_cast<uint32_t>(a.ring)
+                                                  : head % a.ring;
   const int64_t reach = a.max_blocks * a.page_size;
   const uint32_t ps = static_cast<uint32_t>(a.page_size);
+  const auto pages_of = [&](uint32_t x) { return a.log2_page >= 0 ? x >> a.log2_page : x / ps; };
 
-  int64_t tokens = 0, pages = 0;  // of the rows served so far
+  uint32_t tokens = 0, pages = 0;  // of the rows served so far
   bool open = true, found = false;
   uint32_t bits = 0;
-  for (int64_t base = 0; base < a.rows; base += kPlanBlock) {
+  int parity = 0;
+  for (int64_t base = 0; base < a.rows; base += kPlanBlock, parity ^= 1) {
     const int64_t row = base + tid;
     const bool in = row < a.rows;
     const int64_t n_raw = in ? a.new_lens[row] : 0, c = in ? a.cached_lens[row] : 0;
     const bool valid = n_raw >= 0 && c >= 0 && c + n_raw <= reach;
-    const int64_t n = valid ? n_raw : 0;
-    // (32-bit quotients: a valid row's lengths are below 2^31)
-    const uint32_t have = valid ? (static_cast<uint32_t>(c) + ps - 1) / ps : 0u;
-    const uint32_t need = valid ? (static_cast<uint32_t>(c + n) + ps - 1) / ps - have : 0u;
-    int64_t tok = wave_scan(n, lane), pag = wave_scan(static_cast<int64_t>(need), lane);
-    __syncthreads();  // the previous 256 rows' shared values are read
+    const uint32_t n = valid ? static_cast<uint32_t>(n_raw) : 0u;
+    // (a valid row's lengths are at most 2^30)
+    const uint32_t have = valid ? pages_of(static_cast<uint32_t>(c) + ps - 1) : 0u;
+    const uint32_t need = valid ? pages_of(static_cast<uint32_t>(c) + n + ps - 1) - have : 0u;
+    uint32_t tok = wave_scan(n, lane), pag = wave_scan(need, lane);
     if (lane == kWave - 1) {
-      sums[0][wave] = tok;
-      sums[1][wave] = pag;
+      sums[parity][0][wave] = tok;
+      sums[parity][1][wave] = pag;
     }
-    __syncthreads();
+    __syncthreads();  // (and the previous 256 rows' shared values are read)
+    uint32_t tok0 = tokens, pag0 = pages;
 #pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w)
+    for (int w = 0; w < kPlanWaves - 1; ++w)
       if (w < wave) {
-        tok += sums[0][w];
-        pag += sums[1][w];
+        tok0 = add_sat(tok0, sums[parity][0][w]);
+        pag0 = add_sat(pag0, sums[parity][1][w]);
       }
-    tok += tokens;
-    pag += pages;
-    const bool served = open && tok <= a.num_tokens && pag <= avail;
-    const int64_t top_t = wave_max64(served ? tok : 0), top_p = wave_max64(served ? pag : 0);
+    tok = add_sat(tok, tok0);
+    pag = add_sat(pag, pag0);
+    // (the sums grow with the row, so the rows served are the first ones)
+    const bool served = open && tok <= most && pag <= avail;
+    const uint64_t lanes = __builtin_amdgcn_ballot_w64(served);
+    const int last = 63 - __builtin_clzll(lanes | 1);
+    const int top_tok = __builtin_amdgcn_readlane(static_cast<int>(tok), last);
+    const int top_pag = __builtin_amdgcn_readlane(static_cast<int>(pag), last);
     if (lane == 0) {
-      tops[0][wave] = top_t;
-      tops[1][wave] = top_p;
+      tops[0][wave] = lanes != 0 ? top_tok : 0;
+      tops[1][wave] = lanes != 0 ? top_pag : 0;
+      all[wave] = lanes == ~uint64_t{0};
     }
     row_new[tid] = served ? static_cast<int>(n) : 0;
     row_cached[tid] = static_cast<int>(c);
     row_page[tid] = static_cast<int>(served ? pag - need : 0);
-    open = __syncthreads_and(served);
-    const int64_t before = tokens;
+    ends[tid] = served ? static_cast<int>(tok) : INT32_MAX;  // (no token of these rows comes so far)
+    __syncthreads();
+    const uint32_t before = tokens;
 #pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) {
       tokens = max(tokens, tops[0][w]);
       pages = max(pages, tops[1][w]);
+      open = open && all[w] != 0;
     }
-    const int end = static_cast<int>(served ? tok : tokens);
-    ends[tid] = end;
     if (writer && in) {
-      a.cu[row + 1] = end;
+      a.cu[row + 1] = static_cast<int32_t>(served ? tok : tokens);
       a.seq_lens[row] = static_cast<int32_t>(c + (served ? n : 0));
       if (!valid) bits |= MAS_ERRBIT_POSITION;
       else if (!served && n > 0) bits |= MAS_ERRBIT_POOL;
     }
-    __syncthreads();
     if (t >= before && t < tokens) {  // this thread's token lies in these rows
       found = true;
-      int lo = 0, hi = kPlanBlock - 1;  // the first row whose end is past t
+      // the first row whose end is past t: among decode rows, a token each, row t - before; else by halving
+      int lo = static_cast<int>(min(t - before, static_cast<int64_t>(kPlanBlock - 1))), hi = lo;
+      if (ends[lo] <= t || (lo > 0 && ends[lo - 1] > t)) {
+        lo = 0;
+        hi = kPlanBlock - 1;
+      }
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (ends[mid] > t) hi = mid;
@@ -133,7 +155,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_step(StepArgs a) {
       const int64_t r = base + lo;
       const uint32_t cached = static_cast<uint32_t>(row_cached[lo]);
       const uint32_t pos = cached + static_cast<uint32_t>(static_cast<int>(t) - (ends[lo] - row_new[lo]));
-      const uint32_t first = (cached + ps - 1) / ps, block = pos / ps, entry = pos - block * ps;
+      const uint32_t first = pages_of(cached + ps - 1), block = pages_of(pos), entry = pos - block * ps;
       int32_t* const table = a.tables + r * a.bt_stride;
       int32_t page;
       if (block < first) {
@@ -149,7 +171,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_step(StepArgs a) {
       a.slots[t] = page < 0 ? -1 : static_cast<int64_t>(page) * a.page_size + entry;
       if (page < 0) report(a.err, MAS_ERRBIT_PAGE);
     }
-    if (!writer && tokens >= last_t) break;  // uniform: this workgroup's tokens are written
+    if (!writer && (tokens >= last_t || !open)) break;  // uniform: this workgroup's tokens are written
   }
   if (!found && t < a.num_tokens) {  // a padding token
     a.positions[t] = 0;
@@ -192,7 +214,7 @@ extern "C" int mas_plan_step(int32_t* positions, int32_t* batch_indices, int64_t
     return MAS_ERR_UNSUPPORTED;
   const StepArgs a{positions, batch_indices, slot_mapping, cu_seqlens_q, seq_lens, free_range_out, block_tables,
                    block_table_stride, max_blocks, new_lens, cached_lens, rows, free_pages, num_free_pages, free_range,
-                   page_size, num_tokens, err};
+                   page_size, num_tokens, (page_size & (page_size - 1)) == 0 ? __builtin_ctzll(page_size) : -1, err};
   const int64_t blocks = num_tokens > 0 ? cdiv(num_tokens, kPlanBlock) : 1;
   hipLaunchKernelGGL(plan_step, dim3(static_cast<uint32_t>(blocks)), dim3(kPlanBlock), 0, stream, a);
   return launch_status();
