@@ -197,3 +197,46 @@ def test_fp8_output_and_rows_behind_the_last(mas, dev):
     quant = _run(mas, dev, cache, q, tables, lens, cu, 0.1, out_quant_scale=0.03)
     want = (out[:53].float().cpu() / torch.tensor(0.03)).clamp(-448, 448).to(torch.float8_e4m3fn)
     assert torch.equal(quant.cpu().view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dim,pages,layout", [(128, 5 << 20, "HND"), (64, 9 << 20, "NHD")])
+def test_prompts_far_into_a_large_cache(mas, dev, dim, pages, layout):
+    """Byte offsets past 2^32 in the codes: rows stored by slots into the last pages, read back, and attended."""
+    ps, n = 16, 150
+    kv = mas.page.fp4_kv_cache(pages, ps, 1, dim, dev, layout)
+    k, v, q = random_rows(31, n, 1, dim), random_rows(32, n, 1, dim), random_rows(33, 40, 4, dim)
+    order = torch.randperm(12, generator=torch.Generator().manual_seed(4))[:-(-n // ps)]
+    table = (pages - 12 + order)[None].to(torch.int32)
+    p = torch.arange(n)
+    slots = table[0, p // ps].long() * ps + p % ps
+    mas.page.store_kv_slots_fp4(k.to(dev), v.to(dev), kv, slots.to(dev), layout)
+    values = [fp4.dequantize(*fp4.quantize(bits(x))) for x in (k, v)]
+    for got, want in zip(mas.page.load_kv_slots_fp4(kv, slots.to(dev), layout), values):
+        assert np.array_equal(got.float().cpu().numpy(), want)
+    held = []
+    for x in values:
+        few = np.zeros((12, ps, 1, dim))
+        few[order[p // ps].numpy(), (p % ps).numpy()] = x
+        held.append(few)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    out = mas.attention.batch_context_with_fp4_kv_cache(q.to(dev), kv, None, table.to(dev), i32(n), 40, 0, 0.1, 1.0, 1, i32(0, 40),
+                                                        kv_layout=layout)
+    check(out, fp4.context_attention(bits(q), *held, order[None].numpy(), [n], [0, 40], 0.1), n, P_BF16)
+
+
+def test_calls_without_rows(mas, dev):
+    kv = mas.page.fp4_kv_cache(4, 16, 2, 128, dev, "HND")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    none = torch.empty(0, 8, 128, dtype=torch.bfloat16, device=dev)
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device=dev)
+    out = mas.attention.batch_context_with_fp4_kv_cache(none, kv, ws, torch.zeros(0, 3, dtype=torch.int32, device=dev), i32(), 1, 0,
+                                                        0.1, 1.0, 0, i32(0), kv_layout="HND")
+    assert out.shape == none.shape
+    out = mas.attention.batch_decode_with_fp4_kv_cache(none, kv, ws, torch.zeros(0, 3, dtype=torch.int32, device=dev), i32(), 0, 0.1,
+                                                       1.0, kv_layout="HND")
+    assert out.shape == none.shape
+    # rows, but tables of no width: nothing to attend
+    q, flags = random_rows(34, 3, 8, 128).to(dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    out = mas.attention.batch_decode_with_fp4_kv_cache(q, kv, ws, torch.zeros(3, 0, dtype=torch.int32, device=dev), i32(0, 0, 0), 0,
+                                                       0.1, 1.0, out=torch.ones_like(q), kv_layout="HND", error_flags=flags)
+    assert not out.any() and int(flags) == 0
