@@ -1871,7 +1871,9 @@ int context_attention(void* out, int64_t out_stride, int64_t out_head_stride, co
       m.capacity = workspace_bytes;
       m.max_splits = 65535 / num_rows;
       kv_splits = best_splits(m, hint_tiles);
-      if (kv_splits > 1) split_from = split_from_reach(m, hint_tiles);
+      if (kv_splits > 1)
+        split_from = fp4 == nullptr ? split_from_reach(m, hint_tiles)
+                                    : std::max<int64_t>(8, split_tiles(hint_tiles, kv_splits) + 1);
     } else if (base_wgs >= cus && num_rows >= kPlanMinRows && num_rows <= kPlanMaxRows && units_bound <= kPlanMaxUnits &&
                row_tokens <= kPlanMaxTokens && gx <= 32767 && units_bound * tokens_per_wg * num_q_heads <= INT32_MAX) {
       plan = plan_layout(units_bound, gx, resident);
