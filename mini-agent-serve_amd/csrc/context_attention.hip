@@ -97,7 +97,8 @@ struct ContextArgs {
   // indexed by (row * row_tokens + token, head, split); context_combine merges them. Token tiles
   // reaching fewer than split_from key tiles are not split: split 0 computes them whole and writes
   // their output.
-  int kv_splits, row_tokens, split_from;
+  // The merge visits a row's first merge_tokens tokens.
+  int kv_splits, row_tokens, merge_tokens, split_from;
   // The grid launch's order: (head block, row, token tile) with token tiles slowest when set, else
   // (head block, token tile, row) with rows slowest.
   int tile_major;
@@ -644,7 +645,7 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
   // also flagged: a row with more query tokens than the grid covers (max_q_len too small); the
   // tokens past the grid are left unwritten. The planner reports these for planned launches.
   const bool len_bad =
-      !kPlan && (raw_len < q_len || raw_len > cap || q_len > grid_tiles * tokens_per_wg);
+      !kPlan && (raw_len < q_len || raw_len > cap || q_len > (kSplit ? a.merge_tokens : grid_tiles * tokens_per_wg));
   const int kv_len = static_cast<int>(raw_len < 0 ? 0 : (raw_len > cap ? cap : raw_len));
   const int shift = kv_len - q_len;  // position of query token i = shift + i
 
@@ -1442,9 +1443,9 @@ __device__ __forceinline__ void merge_partials(const ContextArgs& a, int64_t bas
 template <int D>
 __global__ __launch_bounds__(64) void context_combine(ContextArgs a, int tokens_per_wg) {
   const int lane = threadIdx.x;
-  const int id = static_cast<int>(blockIdx.x);  // < rows * row_tokens * hq <= 2^31 - 1 (host-checked)
+  const int id = static_cast<int>(blockIdx.x);  // < rows * merge_tokens * hq <= 2^31 - 1 (host-checked)
   const int rt = id / a.hq, h = id - rt * a.hq;
-  const int row = rt / a.row_tokens, t = rt - row * a.row_tokens;
+  const int row = rt / a.merge_tokens, t = rt - row * a.merge_tokens;
   const int q0 = a.cu_seqlens_q[row], q_len = a.cu_seqlens_q[row + 1] - q0;
   if (t >= q_len) return;
   // the token tile's key tiles, as the split kernel counts them
@@ -1846,6 +1847,8 @@ int context_attention(void* out, int64_t out_stride, int64_t out_head_stride, co
   // lays the launch out from the real lengths first: the same estimate on the real grid, one
   // workgroup per item, and a merge over the split tiles only.
   const int64_t row_tokens = gy * tokens_per_wg;
+  // (over the bf16 cache a row of more than max_q_len tokens, up to its last token tile's end, is merged too)
+  const int64_t merge_tokens = fp4 != nullptr ? max_q_len : row_tokens;
   const int64_t entry_bytes = (head_dim + 2) * 4;
   const int64_t units_bound = num_rows * gy;
   int64_t kv_splits = 1, split_from = INT32_MAX;
@@ -1866,7 +1869,7 @@ int context_attention(void* out, int64_t out_stride, int64_t out_head_stride, co
       m.base = base_wgs;
       m.cus = cus;
       m.resident = resident;
-      m.merges = static_cast<double>(num_rows * row_tokens * num_q_heads);
+      m.merges = static_cast<double>(num_rows * merge_tokens * num_q_heads);
       m.partial_per_split = context_partial_bytes(num_rows, row_tokens, num_q_heads, head_dim, 1);
       m.capacity = workspace_bytes;
       m.max_splits = 65535 / num_rows;
@@ -1929,6 +1932,7 @@ int context_attention(void* out, int64_t out_stride, int64_t out_head_stride, co
   a.err = err;
   a.kv_splits = static_cast<int>(kv_splits);
   a.row_tokens = static_cast<int>(row_tokens);
+  a.merge_tokens = static_cast<int>(merge_tokens);
   a.split_from = static_cast<int>(split_from);
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = kv_splits > 1 ? a.part_o + num_rows * row_tokens * num_q_heads * kv_splits * head_dim : nullptr;
@@ -2043,7 +2047,7 @@ int context_attention(void* out, int64_t out_stride, int64_t out_head_stride, co
     launch_context<kWorkGrid>(head_dim, waves, mode, grid, block, stream, a, fp4);
   }
   if (const int st = launch_status(); st != MAS_OK || kv_splits == 1) return st;
-  const int64_t merges = num_rows * row_tokens * num_q_heads;  // <= INT32_MAX when split
+  const int64_t merges = num_rows * merge_tokens * num_q_heads;  // <= INT32_MAX when split
   if (head_dim == 64)
     hipLaunchKernelGGL(context_combine<64>, dim3(static_cast<uint32_t>(merges)), dim3(64), 0, stream, a,
                        static_cast<int>(tokens_per_wg));
