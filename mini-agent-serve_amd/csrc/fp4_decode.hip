@@ -46,7 +46,12 @@ constexpr int kStep = 32;                    // positions a wavefront takes at a
 constexpr int kRound = kWaves * kStep;       // and a workgroup
 constexpr int kMaxSplitLen = 1024;           // positions per split, at most, while max_splits reach
 constexpr int kMaxSplits = 128;
-constexpr int64_t kMaxItems = int64_t{1} << 23;  // workgroups of a launch, at most (a grid is below 2^32 threads)
+// Workgroups of a launch: the splits of a table far wider than its rows are mostly empty, and each costs 1.3 ns. 64 rows of
+// 300 positions under a table of 131072 took 79 us with all 128 splits and 21 with these 8192 workgroups (16384: 29; 4096:
+// 17), rows of 2000 to 4300 99 and 47 (54; 45), one row as long as the table among them 106 and 77 (58; 121).
+constexpr int64_t kMostItems = 8192;
+constexpr int kLongestSplit = 16384;             // positions; as many more workgroups as that takes
+constexpr int64_t kMaxItems = int64_t{1} << 23;  // but no more than this (a grid is below 2^32 threads)
 
 // A row's split length: its share of row_target splits, in whole rounds, at most kMaxSplitLen; and such that its splits
 // fit the grid and the workspace.
@@ -456,16 +461,18 @@ extern "C" int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int
       out_head_stride % 8 != 0 || !aligned16(workspace))
     return MAS_ERR_MISALIGNED;
   // Splits wanted per row: four workgroups per CU over the (row, kv head) pairs. The longest row a table can hold
-  // then has the more of those and of kMaxSplitLen-position splits; fewer where the workspace holds fewer partials.
+  // then has the more of those and of kMaxSplitLen-position splits; fewer where the launch or the workspace would not
+  // hold them.
   int cus = 0;
   if (workspace == nullptr) return MAS_ERR_INVALID_VALUE;
   if (const int st = device_cu_count(&cus); st != MAS_OK) return st;
   const int64_t target = std::max<int64_t>(1, 4 * static_cast<int64_t>(cus) / (batch * num_kv_heads));
   const int64_t held = workspace_bytes / decode_workspace_bytes(batch, num_q_heads, head_dim, 1);
   if (held < 1) return MAS_ERR_INVALID_VALUE;
-  const int64_t splits = std::max<int64_t>(
-      1, std::min({std::max(std::min(target, cdiv(cap, kRound)), cdiv(cap, kMaxSplitLen)), int64_t{kMaxSplits}, held,
-                   kMaxItems / (batch * num_kv_heads)}));
+  const int64_t pairs = batch * num_kv_heads;
+  const int64_t wanted = std::max(std::min(target, cdiv(cap, kRound)), cdiv(cap, kMaxSplitLen));
+  const int64_t launched = std::min(std::max(kMostItems / pairs, cdiv(cap, kLongestSplit)), kMaxItems / pairs);
+  const int64_t splits = std::max<int64_t>(1, std::min({wanted, launched, int64_t{kMaxSplits}, held}));
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_stride;
   a.q_head_stride = q_head_stride;

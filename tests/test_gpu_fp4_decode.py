@@ -238,3 +238,19 @@ def test_as_many_rows_as_a_call_takes(mas, dev):
     want = fp4.decode_attention(bits(q[some]), cache.k, cache.v, tables[some].numpy(), lens[some].tolist(), 0.1)
     check(out[some], want, width * ps, P_TWO_TERMS)
     assert bool(out.isfinite().all())
+
+
+@pytest.mark.parametrize("rows,lens", [(64, [131072, 1, 16385, 300]), (1100, [40000, 20])])
+def test_tables_far_wider_than_the_rows(mas, dev, rows, lens):
+    """A launch holds fewer splits than the table has 1024 positions: a long row's get longer."""
+    ps, width = 256, 512
+    cache = Cache(20, 8, ps, 8, 64, "HND")
+    g = torch.Generator().manual_seed(21)
+    n = torch.randint(0, 300, (rows,), generator=g).to(torch.int32)
+    n[:len(lens)] = torch.tensor(lens, dtype=torch.int32)
+    tables = torch.randint(0, 8, (rows, width), generator=g).to(torch.int32)
+    q = random_rows(22, rows, 8, 64)
+    out = _run(mas, dev, cache, q, tables, n, 0.1, ws_bytes=1 << 30)
+    some = list(range(40))
+    want = fp4.decode_attention(bits(q[some]), cache.k, cache.v, tables[some].numpy(), n[some].tolist(), 0.1)
+    check(out[some], want, max(lens), P_TWO_TERMS)
