@@ -423,7 +423,9 @@ int mas_paged_decode_attention_fp4(void* out, int64_t out_stride, int64_t out_he
 /*
  * Paged causal attention of prompt rows over the 4-bit cache: mas_paged_context_attention_bf16 with the keys
  * and values that the codes stand for (its shapes, masks, workspace and outputs; page_size at least 16). Positions
- * on a page id outside the cache enter as zero keys and values (MAS_ERRBIT_PAGE).
+ * on a page id outside the cache enter as zero keys and values (MAS_ERRBIT_PAGE). A key or value that is NaN or
+ * past bf16's largest number reaches only the tokens that attend to its position; there an element of such a value
+ * gives NaN.
  */
 int mas_paged_context_attention_fp4(void* out, int64_t out_stride, int64_t out_head_stride, const void* q,
                                     int64_t q_stride, int64_t q_head_stride, const void* k_cache, const void* v_cache,

@@ -1311,7 +1311,9 @@ __global__ __launch_bounds__(64 * kWaves, 8 / kWaves) void context_attn(ContextA
       });
     }
     const int t = tok + n;
-    if (hf == 0 && t < q_len) *reinterpret_cast<f32x2*>(a.part_ml + partial(t) * 2) = f32x2{m_run, l_run};
+    // (kPagesFp4: scores that are all NaN leave no maximum; any one makes the merge take the split's NaN in)
+    const float m_out = kFp4 && l_run != l_run && m_run == kNegInf ? 0.f : m_run;
+    if (hf == 0 && t < q_len) *reinterpret_cast<f32x2*>(a.part_ml + partial(t) * 2) = f32x2{m_out, l_run};
     return;
   }
   // ---- out[token][h] = O / l * bmm2_scale (bf16), or its fp8 quantize

@@ -403,7 +403,8 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 3 : 2) void fp4_decode_spli
     } else {
       const int64_t at = (static_cast<int64_t>(b) * a.hq + h) * a.max_splits + split;
       __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(a.part_o + at * D + 4 * c));
-      if (c == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{m_all_lds[g], l};
+      // (scores that are all NaN leave no maximum: any one makes the merge take the split's NaN in)
+      if (c == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{l != l && m_all_lds[g] == kNegInf ? 0.f : m_all_lds[g], l};
     }
   }
 }

@@ -240,3 +240,14 @@ def test_calls_without_rows(mas, dev):
     out = mas.attention.batch_decode_with_fp4_kv_cache(q, kv, ws, torch.zeros(3, 0, dtype=torch.int32, device=dev), i32(0, 0, 0), 0,
                                                        0.1, 1.0, out=torch.ones_like(q), kv_layout="HND", error_flags=flags)
     assert not out.any() and int(flags) == 0
+
+
+@pytest.mark.parametrize("rows,ws_bytes", [([(8, 3000)], 64 << 20), ([(8, 3000)], 0), ([(8, 3000)] + [(3, 40)] * 16, 64 << 20)])
+def test_a_nan_query_shows(mas, dev, rows, ws_bytes):
+    """In a call that splits its key range, one that does not, and one laid out on the device."""
+    cache, q, tables, lens, cu = _case(35, 8, 2, 128, 16, "HND", rows)
+    q[3, 5, 17] = float("nan")
+    out = _run(mas, dev, cache, q, tables, lens, cu, 0.1, ws_bytes=ws_bytes, max_q=512 if len(rows) > 1 else None).cpu()
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[3, 5] = True
+    assert bool(out[bad].isnan().all()) and bool(out[~bad].isfinite().all())

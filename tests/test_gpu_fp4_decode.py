@@ -254,3 +254,23 @@ def test_tables_far_wider_than_the_rows(mas, dev, rows, lens):
     some = list(range(40))
     want = fp4.decode_attention(bits(q[some]), cache.k, cache.v, tables[some].numpy(), n[some].tolist(), 0.1)
     check(out[some], want, max(lens), P_TWO_TERMS)
+
+
+@pytest.mark.parametrize("where", ["key", "value", "query"])
+def test_a_nan_shows_through_the_merge(mas, dev, where):
+    """As above, in rows of several splits; a NaN query makes every split's scores NaN."""
+    cache, q, tables, n = _case(23, 8, 2, 128, 16, "HND", [3000, 2500])
+    page = int(tables[1, 60])
+    if where == "query":
+        q[1, 5, 17] = float("nan")
+    else:
+        cache.tensors[2 if where == "key" else 3][page, 1, 2, 4] = 255
+    out = _run(mas, dev, cache, q, tables, n, 0.1).cpu()
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    if where == "query":
+        bad[1, 5] = True
+    elif where == "key":
+        bad[1, 4:] = True
+    else:
+        bad[1, 4:, 64:96] = True
+    assert bool(out[bad].isnan().all()) and bool(out[~bad].isfinite().all())
