@@ -251,3 +251,15 @@ def test_a_nan_query_shows(mas, dev, rows, ws_bytes):
     bad = torch.zeros_like(out, dtype=torch.bool)
     bad[3, 5] = True
     assert bool(out[bad].isnan().all()) and bool(out[~bad].isfinite().all())
+
+
+def test_more_tokens_than_max_q_len(mas, dev):
+    """A row of more tokens than the call says, its key range split: reported, and the tokens past max_q_len stay."""
+    cache, q, tables, lens, cu = _case(36, 8, 2, 128, 16, "HND", [(8, 3000), (5, 2000)])
+    flags = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = torch.full(q.shape, 3.0, dtype=torch.bfloat16, device=dev)
+    _run(mas, dev, cache, q, tables, lens, cu, 0.1, max_q=5, out=out, error_flags=flags)
+    assert int(flags) == 2 and bool((out[5:8] == 3).all())
+    kept = list(range(5)) + list(range(8, 13))
+    want = fp4.context_attention(bits(q), cache.k, cache.v, tables.numpy(), lens, cu, 0.1)
+    check(out[kept], (want[0][kept], want[1][kept], want[2]), 3000, P_BF16)
