@@ -15,8 +15,8 @@
 // One thread per token, and every workgroup sums the rows' tokens and pages itself, 256 rows at a time (a row
 // per thread, both sums in one pass of wavefront scans), until its own tokens are covered: no workgroup
 // waits for another, and one launch does it. What bounds it: the latencies of the lengths, the page and the stores.
-// 256 decode rows 3.2 us, 64 decode rows and 8 prompts (8384 tokens) 4.1 us, of which an empty launch is about half. With 64-bit
-// shuffled scans, four barriers and a search for every token: 4.4 and 5.1 us.
+// 256 decode rows 3.2 us, 64 decode rows and 8 prompts (8384 tokens) 4.1 us; with 64-bit shuffled scans, four barriers and
+// a search for every token 4.4 and 5.1 us.
 #include <type_traits>
 
 #include "device.h"
